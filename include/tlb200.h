@@ -241,6 +241,96 @@ tlb_status tlb_paged_attention_static(tlb_device *dev, const void *q, const void
                                       int heads, int kv_heads, int head_size, int block_size, int max_blocks,
                                       int max_context, float scale);
 
+/* ------------------------------------------------------------------ serving operators on device arrays
+ * No counterpart in the reference. What a server needs beside the paged decode step: the prompts of a batch in one pass without padding,
+ * several drafted tokens per sequence verified in one pass over the cache (speculative decoding), the accepted ones moved into place, and
+ * the scores of tokens. The same operators are graph nodes (PACKED_ATTN, PAGED_TREE_ATTENTION, TOKEN_LOGPROBS) with the planner's scratch.
+ *
+ * Every pointer is device memory of the handle's device unless a comment says otherwise; strides are bytes. `stream` is a cudaStream_t of that
+ * device, NULL for the device's own (tlb_device_stream); the legacy default stream is cudaStreamLegacy, (void *)1. The calls enqueue and
+ * return: nothing is allocated, waited for or kept, and they may be captured into a CUDA graph. `workspace` (16-byte aligned, of at least the size
+ * that the _workspace function gives for the same shapes) needs no initial content; calls that may overlap in time need one each.
+ * Shapes and alignments are checked (TLB_INVALID, TLB_UNSUPPORTED); numbers in device memory are checked where they are read: one that
+ * points outside is not followed, and *status (device or pinned memory, may be NULL, never reset) becomes 4; it becomes 2 if a kernel gave up
+ * waiting for its own copies. Outputs may not overlap inputs. */
+
+/* Causal attention over packed sequences: sequence s has the query rows q_offsets[s] .. q_offsets[s + 1] and the key rows kv_offsets[s] ..
+ * kv_offsets[s + 1]; its last query sees all of its keys, the one before it one less, ... (as many keys as queries: a prompt; more: a chunk
+ * behind keys of earlier tokens; fewer: the first queries see nothing and give zeros). Query head h reads KV head h / (heads / kv_heads).
+ * Head sizes: multiples of 8 up to 512 (tuned up to 128). Rows outside every sequence stay as they were, and so do those of a sequence whose
+ * offsets fall or reach outside the rows (reported). */
+typedef struct tlb_packed_attention_args {
+    uint32_t type;                    /* of q, k, v, out: TLB_TYPE_F16 or TLB_TYPE_BF16 */
+    uint32_t seqs, heads, kv_heads, head_size;
+    float scale;                      /* of the scores, positive; usually 1 / sqrt(head_size) */
+    uint64_t q_rows, kv_rows;         /* rows that q and out hold, and k and v */
+    const void *q, *k, *v;            /* rows of [heads][head_size]; 16-byte aligned */
+    void *out;
+    uint64_t q_stride, k_stride, v_stride, out_stride;   /* from row to row, multiples of 16 */
+    const int32_t *q_offsets, *kv_offsets;               /* seqs + 1 each; kv_offsets NULL: the same as q_offsets */
+    void *workspace;
+    uint64_t workspace_bytes;
+    int32_t *status;
+} tlb_packed_attention_args;
+uint64_t   tlb_packed_attention_workspace(tlb_device *dev, const tlb_packed_attention_args *args);   /* pointers are not looked at */
+tlb_status tlb_packed_attention(tlb_device *dev, const tlb_packed_attention_args *args, void *stream);
+
+/* Attention of drafted tokens over the paged cache. Sequence s has context[s] tokens in the cache and counts[s] <= drafts drafted tokens behind
+ * them, whose keys and values the cache holds too (positions context[s] + i of the block table). Draft i sees the context, itself and
+ * its ancestors: parents[s][i] is an earlier draft of the sequence, or -1 where it follows the context directly. f16; rows of q and out
+ * from counts[s] on are padding, zero in out. 1 to 64 drafts per sequence. */
+typedef struct tlb_tree_attention_args {
+    uint32_t seqs, drafts, heads, kv_heads, head_size, block_size, max_blocks;
+    float scale;
+    uint64_t pool_blocks;
+    const void *q;                    /* [seqs][drafts][heads][head_size] */
+    const void *k_pool, *v_pool;      /* [pool_blocks][kv_heads][block_size][head_size], as the cache-write node fills them */
+    void *out;                        /* as q */
+    const int32_t *tables;            /* [seqs][max_blocks] */
+    const int32_t *context, *counts;  /* [seqs] */
+    const int32_t *parents;           /* [seqs][drafts] */
+    void *workspace;
+    uint64_t workspace_bytes;
+    int32_t *status;
+} tlb_tree_attention_args;
+uint64_t   tlb_tree_attention_workspace(tlb_device *dev, const tlb_tree_attention_args *args);
+tlb_status tlb_tree_attention(tlb_device *dev, const tlb_tree_attention_args *args, void *stream);
+
+/* Moves the accepted drafts into place in the pools of all layers: for j < counts[s], position context[s] + path[s][j] goes to position
+ * context[s] + j. path[s] rises strictly (a path from the context to a leaf). A sequence whose numbers point outside is left as it was
+ * (reported). Sequences may not share the pages they write to. */
+typedef struct tlb_cache_keep_args {
+    uint32_t layers, seqs, drafts, kv_heads, head_size, block_size, max_blocks;
+    uint64_t pool_blocks;
+    void *k_pools, *v_pools;          /* of the first layer */
+    uint64_t k_layer_stride, v_layer_stride;   /* from layer to layer, multiples of 16 */
+    const int32_t *tables;            /* [seqs][max_blocks] */
+    const int32_t *context, *counts;  /* [seqs] */
+    const int32_t *path;              /* [seqs][drafts] */
+    int32_t *status;
+} tlb_cache_keep_args;
+tlb_status tlb_cache_keep(tlb_device *dev, const tlb_cache_keep_args *args, void *stream);
+
+/* Of each row of logits: the log probability of tokens[row] (-1: none, 0 is written), the entropy in nats, and the `top` (up to 32) most likely
+ * tokens with their log probabilities, equal logits by rising id. Tokens at -inf have no part in the entropy and are not listed (ids -1 at
+ * -inf where fewer are left). A row that holds a NaN or +inf gives NaN and ids of -1; a row of -inf alone gives -inf, and entropy 0. */
+typedef struct tlb_token_logprobs_args {
+    uint32_t type;                    /* TLB_TYPE_F32, TLB_TYPE_F16 or TLB_TYPE_BF16 */
+    uint32_t top;
+    uint64_t rows, vocab;
+    const void *logits;               /* rows of vocab values */
+    uint64_t stride;                  /* from row to row, a multiple of the value's size */
+    const int32_t *tokens;            /* [rows]; NULL: none */
+    float *logprob, *entropy;         /* [rows]; may be NULL */
+    int32_t *top_ids;                 /* [rows][top]; may be NULL where top is 0 */
+    float *top_logprobs;
+    void *workspace;
+    uint64_t workspace_bytes;
+    int32_t *status;
+} tlb_token_logprobs_args;
+uint64_t   tlb_token_logprobs_workspace(tlb_device *dev, const tlb_token_logprobs_args *args);
+tlb_status tlb_token_logprobs(tlb_device *dev, const tlb_token_logprobs_args *args, void *stream);
+
 /* ------------------------------------------------------------------ tensor parallelism
  * No counterpart in the reference (single device: model.rs:415-422). A communicator joins the
  * ranks of one box; programs compiled on a device with a communicator may contain the pseudo-op

@@ -62,6 +62,25 @@ class tlb_leaves(C.Structure):
     ]
 
 
+def _struct(name, *fields):
+    return type(name, (C.Structure,), {"_fields_": [(f, ty) for ty, names in fields for f in names.split()]})
+
+
+_U32, _U64, _F32, _PTR = C.c_uint32, C.c_uint64, C.c_float, C.c_void_p
+tlb_packed_attention_args = _struct(
+    "tlb_packed_attention_args", (_U32, "type seqs heads kv_heads head_size"), (_F32, "scale"), (_U64, "q_rows kv_rows"), (_PTR, "q k v out"),
+    (_U64, "q_stride k_stride v_stride out_stride"), (_PTR, "q_offsets kv_offsets workspace"), (_U64, "workspace_bytes"), (_PTR, "status"))
+tlb_tree_attention_args = _struct(
+    "tlb_tree_attention_args", (_U32, "seqs drafts heads kv_heads head_size block_size max_blocks"), (_F32, "scale"), (_U64, "pool_blocks"),
+    (_PTR, "q k_pool v_pool out tables context counts parents workspace"), (_U64, "workspace_bytes"), (_PTR, "status"))
+tlb_cache_keep_args = _struct(
+    "tlb_cache_keep_args", (_U32, "layers seqs drafts kv_heads head_size block_size max_blocks"), (_U64, "pool_blocks"), (_PTR, "k_pools v_pools"),
+    (_U64, "k_layer_stride v_layer_stride"), (_PTR, "tables context counts path status"))
+tlb_token_logprobs_args = _struct(
+    "tlb_token_logprobs_args", (_U32, "type top"), (_U64, "rows vocab"), (_PTR, "logits"), (_U64, "stride"),
+    (_PTR, "tokens logprob entropy top_ids top_logprobs workspace"), (_U64, "workspace_bytes"), (_PTR, "status"))
+
+
 # every symbol include/tlb200.h declares: name -> (restype, argtypes)
 _P = C.c_void_p
 SYMBOLS = {
@@ -107,6 +126,13 @@ SYMBOLS = {
     "tlb_row_size": (C.c_uint64, [C.c_uint32, C.c_int64]),
     "tlb_paged_attention_static": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                             C.c_int, C.c_float]),
+    "tlb_packed_attention_workspace": (C.c_uint64, [_P, _P]),
+    "tlb_packed_attention": (C.c_int, [_P, _P, _P]),
+    "tlb_tree_attention_workspace": (C.c_uint64, [_P, _P]),
+    "tlb_tree_attention": (C.c_int, [_P, _P, _P]),
+    "tlb_cache_keep": (C.c_int, [_P, _P, _P]),
+    "tlb_token_logprobs_workspace": (C.c_uint64, [_P, _P]),
+    "tlb_token_logprobs": (C.c_int, [_P, _P, _P]),
     "tlb_comm_unique_id": (C.c_int, [_P]),
     "tlb_comm_init": (C.c_int, [_P, C.c_int, C.c_int, _P]),
     "tlb_comm_destroy": (C.c_int, [_P]),

@@ -317,4 +317,55 @@ cudaError_t launch_paged_gather(int seqs, int kv_heads, int hs, int block_size, 
                                 int max_ctx, cudaStream_t st);
 void attn_configure();
 
+// ---------------------------------------------------------------- k_serve_attn.cu, k_serve_attn_tc.cu
+// Causal attention over packed sequences (PACKED_ATTN) and attention of drafted tokens over the paged cache (PAGED_TREE_ATTN).
+// Tokens are rows of [head][head size]; strides are bytes from one token to the next.
+struct ServeAttn {
+    bool paged, bf16;              // paged: the pools of k_attn.cu (f16), else rows of f16 or bf16
+    int seqs, heads, kv_heads, hs;
+    float scale;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride, q_rows;
+    const void *k, *v;             // rows, or the pools
+    int64_t k_stride, v_stride, kv_rows;
+    const int32_t *q_off, *kv_off; // packed: seqs + 1 each
+    const int32_t *tables, *context, *counts, *parents;   // paged
+    int drafts, block_size, max_blocks;
+    int64_t pool_blocks;
+    int *err;                      // may be null
+};
+constexpr int TREE_MAX_DRAFTS = 64;   // a token's ancestors are a 64-bit mask
+const char *serve_attn_refusal(const ServeAttn &a);   // why the shapes are not supported, or null
+uint64_t serve_attn_scratch_bytes(const ServeAttn &a, int sm_count);
+cudaError_t launch_serve_attn(const ServeAttn &a, void *scratch, int sm_count, cudaStream_t st);
+// The accepted drafts of every sequence (their places among the drafts, rising) to positions context, context + 1, ... in the pools of all layers
+struct CacheKeep {
+    void *kpool, *vpool;           // of the first layer
+    int64_t k_layer, v_layer;      // bytes from layer to layer
+    int layers, kv_heads, hs, block_size, seqs, max_blocks, drafts;
+    int64_t pool_blocks;
+    const int32_t *tables, *context, *path, *counts;
+    int *err;
+};
+cudaError_t launch_cache_keep(const CacheKeep &a, cudaStream_t st);
+
+// ---------------------------------------------------------------- k_logprobs.cu
+// Of each row of logits: log probability of a given token, entropy, the most likely tokens (ties: the lowest id) with theirs
+constexpr int LOGPROBS_MAX_TOP = 32;
+struct Logprobs {
+    uint32_t type;                 // f32, f16 or bf16
+    int64_t rows, vocab, stride;   // stride: bytes
+    int top;
+    const void *logits;
+    const int32_t *tokens;         // null: none
+    float *logprob, *entropy, *top_logprobs;   // logprob and entropy may be null
+    void *top_ids;                 // i32, or f32 (ids_f32)
+    int64_t out_step, top_step;    // elements from row to row: of logprob and entropy, of the two top arrays
+    bool ids_f32;
+    int *err;
+};
+uint64_t logprobs_scratch_bytes(const Logprobs &a, int sm_count);
+cudaError_t launch_logprobs(const Logprobs &a, void *scratch, int sm_count, cudaStream_t st);
+
 }  // namespace tlb

@@ -1002,6 +1002,148 @@ void lower_allreduce(L &l) {
         return comm_allreduce_f32(dev, (float *)r.at(pd), n, r.stream, r.err);
     });
 }
+// ---- PACKED_ATTN, PAGED_TREE_ATTENTION, TOKEN_LOGPROBS: serving operators without a counterpart in ggml (include/tlb200.h describes them)
+// The kernel arguments of an attention node without its addresses, or a reason why it is not supported
+static const char *serve_attn_args(const Graph &g, const Tensor &t, ServeAttn &a) {
+    const bool paged = t.op == "PAGED_TREE_ATTENTION";
+    for (int i = 0; i < (paged ? 7 : 4); i++)
+        if (t.src[i] < 0) return "missing operands";
+    const Tensor &q = g.tensors[t.src[0]], &k = g.tensors[t.src[1]], &v = g.tensors[t.src[2]];
+    auto numbers = [&](int i, int64_t n) {
+        const Tensor &x = g.tensors[t.src[i]];
+        return x.ty == TLB_TYPE_I32 && x.is_contiguous() && x.nelements() == n;
+    };
+    auto heads_dense = [](const Tensor &x) {   // rows of [head][head size], a multiple of 16 bytes apart
+        return x.nb[0] == 2 && x.nb[1] == (uint64_t)x.ne[0] * 2 && x.nb[2] % 16 == 0 && x.nb[2] >= (uint64_t)x.ne[0] * x.ne[1] * 2 && x.ne[3] == 1 && x.view_offs % 16 == 0;
+    };
+    a = ServeAttn{};
+    a.paged = paged;
+    a.bf16 = q.ty == TLB_TYPE_BF16;
+    a.scale = t.param_f32(0);
+    a.hs = (int)q.ne[0];
+    a.heads = (int)q.ne[1];
+    if (t.ty != q.ty || k.ty != q.ty || v.ty != q.ty || (q.ty != TLB_TYPE_F16 && q.ty != TLB_TYPE_BF16)) return "queries, keys, values and result must all be f16 or all bf16";
+    for (int i = 0; i < 4; i++)
+        if (t.ne[i] != q.ne[i]) return "the result has the shape of the queries";
+    if (!t.is_contiguous()) return "the result must be contiguous";
+    if (paged) {
+        a.kv_heads = t.op_params[1];
+        a.block_size = t.op_params[2];
+        a.drafts = (int)q.ne[2];
+        a.seqs = (int)q.ne[3];
+        a.max_blocks = (int)g.tensors[t.src[3]].ne[0];
+        if (!q.is_contiguous() || q.view_offs % 16 || k.view_offs % 16 || v.view_offs % 16) return "the queries must be contiguous";
+        if (!k.is_contiguous() || !v.is_contiguous()) return "the pools must be contiguous";
+        if (!numbers(3, (int64_t)a.max_blocks * a.seqs) || !numbers(4, a.seqs) || !numbers(5, a.seqs) || !numbers(6, (int64_t)a.drafts * a.seqs))
+            return "block tables, context lengths, counts and parents must be contiguous i32, one row or number per sequence";
+        if (a.kv_heads < 1 || a.block_size < 1 || a.hs < 1) return "the query heads must be a multiple of the kv heads";
+        a.pool_blocks = std::min(k.nelements(), v.nelements()) / ((int64_t)a.kv_heads * a.block_size * a.hs);
+        a.q_rows = (int64_t)a.drafts * a.seqs;
+        a.q_stride = a.out_stride = (int64_t)a.heads * a.hs * 2;
+    } else {
+        a.kv_heads = (int)k.ne[1];
+        a.seqs = (int)g.tensors[t.src[3]].nelements() - 1;
+        if (!heads_dense(q) || !heads_dense(k) || !heads_dense(v)) return "rows must be dense and lie a multiple of 16 bytes apart";
+        if (k.ne[0] != q.ne[0] || v.ne[0] != q.ne[0] || v.ne[1] != k.ne[1] || v.ne[2] != k.ne[2]) return "inconsistent shapes";
+        if (a.seqs < 0 || !numbers(3, a.seqs + 1) || (t.src[4] >= 0 && !numbers(4, a.seqs + 1))) return "offsets must be contiguous i32, sequences + 1 of them";
+        if (t.src[4] < 0 && k.ne[2] != q.ne[2]) return "keys of another number than the queries need offsets of their own";
+        a.q_rows = q.ne[2];
+        a.kv_rows = k.ne[2];
+        a.q_stride = (int64_t)q.nb[2];
+        a.k_stride = (int64_t)k.nb[2];
+        a.v_stride = (int64_t)v.nb[2];
+        a.out_stride = (int64_t)t.nb[2];
+    }
+    return serve_attn_refusal(a);
+}
+
+void lower_serve_attn(L &l) {
+    const Tensor &t = l.t();
+    ServeAttn a;
+    if (const char *why = serve_attn_args(*l.c.g, t, a)) unsupported(t, why);
+    const int sm = l.c.dev->prop.multiProcessorCount;
+    Place p[7], ps;
+    for (int i = 0; i < 7; i++)
+        if (t.src[i] >= 0) p[i] = l.place(t.src[i]);
+    const bool own_kv_off = t.src[4] >= 0;
+    if (serve_attn_scratch_bytes(a, sm) > 0) {
+        const int64_t sc = l.c.layout->scratch[l.pos];
+        if (sc < 0) throw std::string("attention scratch was not planned");
+        ps.buf = BUF_ARENA;
+        ps.off = (uint64_t)sc;
+    }
+    const Place pd = l.place(l.id);
+    const Place q = p[0], k = p[1], v = p[2], n3 = p[3], n4 = p[4], n5 = p[5], n6 = p[6];
+    l.push([=](const RunCtx &r) {
+        ServeAttn x = a;
+        x.q = r.at(q);
+        x.k = r.at(k);
+        x.v = r.at(v);
+        x.out = r.at(pd);
+        x.err = r.err;
+        if (x.paged) {
+            x.tables = (const int32_t *)r.at(n3);
+            x.context = (const int32_t *)r.at(n4);
+            x.counts = (const int32_t *)r.at(n5);
+            x.parents = (const int32_t *)r.at(n6);
+        } else {
+            x.q_off = (const int32_t *)r.at(n3);
+            x.kv_off = own_kv_off ? (const int32_t *)r.at(n4) : x.q_off;
+        }
+        return launch_serve_attn(x, r.at(ps), sm, r.stream);
+    });
+}
+
+static const char *logprobs_args(const Graph &g, const Tensor &t, Logprobs &a) {
+    if (t.src[0] < 0) return "missing operands";
+    const Tensor &x = g.tensors[t.src[0]];
+    a = Logprobs{};
+    a.type = x.ty;
+    a.top = t.op_params[0];
+    a.vocab = x.ne[0];
+    a.rows = x.ne[1];
+    a.stride = (int64_t)x.nb[1];
+    if (x.ty != TLB_TYPE_F32 && x.ty != TLB_TYPE_F16 && x.ty != TLB_TYPE_BF16) return "logits must be f32, f16 or bf16";
+    if (x.ne[2] * x.ne[3] != 1 || x.nb[0] != type_traits(x.ty)->size || x.nb[1] < x.nb[0] * (uint64_t)x.ne[0] || x.nb[1] % x.nb[0]) return "logits must be rows of dense values";
+    if (a.top < 0 || a.top > LOGPROBS_MAX_TOP) return "at most 32 alternatives";
+    if (a.vocab > (1 << 24) || a.rows > 0x7fffffff) return "ids above 2^24 are no f32 values";   // the node's result holds them as such
+    if (t.ty != TLB_TYPE_F32 || !t.is_contiguous() || t.ne[0] != 2 + 2 * a.top || t.ne[1] != a.rows || t.ne[2] * t.ne[3] != 1) return "the result must be f32 [2 + 2 top, rows]";
+    if (t.src[1] >= 0) {
+        const Tensor &k = g.tensors[t.src[1]];
+        if (k.ty != TLB_TYPE_I32 || !k.is_contiguous() || k.nelements() != a.rows) return "one i32 token per row";
+    }
+    a.out_step = a.top_step = t.ne[0];
+    a.ids_f32 = true;
+    return nullptr;
+}
+
+void lower_logprobs(L &l) {
+    const Tensor &t = l.t();
+    Logprobs a;
+    if (const char *why = logprobs_args(*l.c.g, t, a)) unsupported(t, why);
+    const int sm = l.c.dev->prop.multiProcessorCount;
+    const int64_t sc = l.c.layout->scratch[l.pos];
+    if (sc < 0) throw std::string("logprobs scratch was not planned");
+    Place ps, pt;
+    ps.buf = BUF_ARENA;
+    ps.off = (uint64_t)sc;
+    const bool has_tokens = t.src[1] >= 0;
+    if (has_tokens) pt = l.place(t.src[1]);
+    const Place px = l.place(t.src[0]), pd = l.place(l.id);
+    l.push([=](const RunCtx &r) {
+        Logprobs x = a;
+        float *o = (float *)r.at(pd);
+        x.logits = r.at(px);
+        x.tokens = has_tokens ? (const int32_t *)r.at(pt) : nullptr;
+        x.logprob = o;
+        x.entropy = o + 1;
+        x.top_ids = o + 2;
+        x.top_logprobs = o + 2 + x.top;
+        x.err = r.err;
+        return launch_logprobs(x, r.at(ps), sm, r.stream);
+    });
+}
+
 
 }  // namespace
 
@@ -1018,6 +1160,14 @@ uint64_t node_scratch_bytes(const Graph &g, int32_t id, int sm_count) {
             flash_split_plan(p, sm_count);
             return flash_split_scratch_bytes(p);
         }
+    }
+    if (t.op == "PACKED_ATTN" || t.op == "PAGED_TREE_ATTENTION") {
+        ServeAttn a;
+        if (serve_attn_args(g, t, a) == nullptr) return serve_attn_scratch_bytes(a, sm_count);
+    }
+    if (t.op == "TOKEN_LOGPROBS") {
+        Logprobs a;
+        if (logprobs_args(g, t, a) == nullptr) return logprobs_scratch_bytes(a, sm_count);
     }
     if (t.op == "MUL_MAT_GROUP") {
         const Tensor &tx = g.tensors[t.src[1]];
@@ -1186,6 +1336,8 @@ void lower_node(const LowerCtx &c, int32_t id, int pos, std::vector<Dispatch> &o
     if (op == "CUSTOM") return lower_custom(l);
     if (op == "FLASH_ATTN_EXT") return lower_flash(l);
     if (op == "ALLREDUCE") return lower_allreduce(l);
+    if (op == "PACKED_ATTN" || op == "PAGED_TREE_ATTENTION") return lower_serve_attn(l);
+    if (op == "TOKEN_LOGPROBS") return lower_logprobs(l);
     unsupported(t, "op not implemented in the native CUDA backend");
 }
 

@@ -442,6 +442,28 @@ class Graph:
     def allreduce(self, a: int, name: str = "") -> int:
         return self._node(self._view(a), "ALLREDUCE", [a], name=name or "allreduce")
 
+    # serving operators (no ggml counterpart; include/tlb200.h, "serving operators", says what each computes)
+    def packed_attention(self, q: int, k: int, v: int, q_offsets: int, scale: float, kv_offsets: int | None = None, name: str = "") -> int:
+        """Causal attention over packed sequences: q [hs, heads, rows], k and v [hs, kv heads, rows] (f16 or bf16), offsets i32 [sequences + 1];
+        the result has q's shape and type. Rows of no sequence are not written."""
+        Q, K = self.tensors[q], self.tensors[k]
+        assert Q.ne[0] == K.ne[0] and Q.ne[1] % K.ne[1] == 0 and self.tensors[v].ne == K.ne and Q.ne[3] == 1 and scale > 0
+        return self._node(self._dup(q), "PACKED_ATTN", [q, k, v, q_offsets, kv_offsets], {0: f32_bits(scale)}, name or "packed_attention")
+
+    def paged_tree_attention(self, q: int, kc: int, vc: int, tables: int, context: int, counts: int, parents: int, block_size: int, scale: float,
+                             kv_heads: int = 1, name: str = "") -> int:
+        """Drafted tokens over the paged cache: q f16 [hs, heads, drafts, sequences], tables i32 [pages, sequences], context and counts
+        i32 [sequences], parents i32 [drafts, sequences]; the result has q's shape."""
+        assert self.tensors[q].ne[1] % kv_heads == 0 and scale > 0
+        return self._node(self._dup(q), "PAGED_TREE_ATTENTION", [q, kc, vc, tables, context, counts, parents],
+                          {0: f32_bits(scale), 1: kv_heads, 2: block_size}, name or "paged_tree_attention")
+
+    def token_logprobs(self, logits: int, tokens: int | None, top: int = 0, name: str = "") -> int:
+        """f32 [2 + 2 top, rows] of logits [vocabulary, rows]: the log probability of the row's token (i32; -1 or None: 0), the entropy, the ids of
+        the `top` most likely tokens (as f32; -1 where there are none left) and their log probabilities."""
+        t = self._new(F32, [2 + 2 * top, self.tensors[logits].ne[1]])
+        return self._node(t, "TOKEN_LOGPROBS", [logits, tokens], {0: top}, name)
+
     # ------------------------------------------------------------------ C structs
     def to_c(self):
         """(tlb_graph, keepalive) for tlb_program_compile."""

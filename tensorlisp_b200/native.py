@@ -125,6 +125,7 @@ class Native:
         h = C.c_void_p()
         check(self.L.tlb_device_open(ordinal, C.byref(h)))
         self.dev = h
+        self.ordinal = ordinal
         self.weights: StateBlock | None = None
         self.weight_loc: list[tuple[int, int]] = []   # weight index -> (buffer index, byte offset)
         self.state: StateBlock | None = None
