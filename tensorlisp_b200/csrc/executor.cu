@@ -227,6 +227,7 @@ static void configure_kernels_once(int ordinal) {
     mm_plain_configure();
     mm_q6_configure();
     flash_tc_configure();
+    serve_attn_tc_configure();
     g_configured_ordinals |= bit;
 }
 

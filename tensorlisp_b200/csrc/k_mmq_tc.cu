@@ -711,6 +711,23 @@ void launch_mmq_reduce(const float *partial, float *y, int64_t total, int n_spli
     launch_reduce_segs(partial, g, total, n_split, st);
 }
 
+// Tensor map of f16 or bf16 with two or three dimensions (strides of the outer ones in bytes), boxes of 64 elements by box[1] (by box[2]) with the
+// 128-byte swizzle; what lies outside reads as zero
+cudaError_t tc_encode_sw128(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides, const uint32_t *box, bool bf16) {
+    if (encode_tiled() == nullptr) return cudaErrorNotSupported;
+    cuuint64_t gdim[3] = {1, 1, 1}, gstride[2] = {16, 16};
+    cuuint32_t bx[3] = {1, 1, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    for (int i = 0; i < rank; i++) {
+        gdim[i] = dims[i];
+        bx[i] = box[i];
+        if (i) gstride[i - 1] = strides[i - 1];
+    }
+    return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void *>(base), gdim, gstride, bx, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 bool tc_available() { return encode_tiled() != nullptr; }
 
 // Test hook: every thread of one CTA waits, with the kernels' own bounded wait, on a barrier that nothing ever

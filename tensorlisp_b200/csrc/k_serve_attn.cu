@@ -147,9 +147,12 @@ static cudaError_t launch_any(const ServeAttn &a, cudaStream_t st) {
     const dim3 grid((unsigned)a.q_rows, (unsigned)a.heads);
     return a.hs <= 256 ? launch_pdl(k_serve_attn_any<T, PAGED, 1>, grid, dim3(128), 0, st, a) : launch_pdl(k_serve_attn_any<T, PAGED, 2>, grid, dim3(128), 0, st, a);
 }
-uint64_t serve_attn_scratch_bytes(const ServeAttn &, int) { return 0; }
-cudaError_t launch_serve_attn(const ServeAttn &a, void *, int, cudaStream_t st) {
+uint64_t serve_attn_scratch_bytes(const ServeAttn &a, int sm_count) {
+    return a.q_rows && a.seqs && serve_attn_tc_supported(a) ? serve_attn_tc_scratch_bytes(a, sm_count) : 0;
+}
+cudaError_t launch_serve_attn(const ServeAttn &a, void *scratch, int sm_count, cudaStream_t st) {
     if (a.q_rows == 0 || a.seqs == 0) return cudaSuccess;
+    if (serve_attn_tc_supported(a)) return launch_serve_attn_tc(a, scratch, sm_count, st);
     if (a.paged) return launch_any<__half, true>(a, st);
     return a.bf16 ? launch_any<__nv_bfloat16, false>(a, st) : launch_any<__half, false>(a, st);
 }

@@ -1,0 +1,874 @@
+// The attention of k_serve_attn.cu on the 5th-generation tensor cores: head sizes up to 128, f16 or bf16.
+//
+// A tile of 128 rows holds `tpt` tokens x the query heads of one KV head (token by token, so a short sequence or a few drafts fill it as
+// well as they can), a key tile 128 keys. Keys and values come by TMA from where they lie (rows of any stride, or pages), 128-byte
+// swizzled; V is read as the MN-major operand, so nothing is packed or transposed first. Columns past the head size and rows past the
+// tensors are filled with zeros by the copy.
+//
+//   S = Q K^T (f32, tensor memory),  P = 2^(scale S - m) in the inputs' type, written over S,  O += P V (f32, tensor memory)
+//
+// Two streams of S and O per CTA keep the tensor core busy while the exponentials of the other one are taken:
+//   SHARE  a pair of row tiles against every key tile (prompts)
+//   else   one row tile, key tiles in turn; the two O are joined at the end (drafts, chunks of few tokens: bound by the keys' bytes)
+// Each has four warps, a thread per row. The maximum m that a row's exponents refer to moves when a tile's maximum has outgrown it by 2^8
+// (the factor cancels; P stays far inside f16), so O is rescaled rarely. The row sums add P as it was rounded, so a dominant key's rounding
+// cancels.
+//
+// Work is shared out evenly: the units are (row tile, KV head, key tile), in one line over all sequences, and every CTA takes an equal
+// stretch of it (one persistent CTA per SM). Row tiles that are cut leave (m, l, O) in the workspace and k_serve_join adds them up. Lengths
+// are read on the device, so the same launch serves any batch.
+//
+// Tiles at the diagonal, at the end of a sequence or in the tree are `special`: scores are masked by index, and because 0 x NaN is not 0,
+// two warps look through their values first: rows behind the sequence's end become zero, and where a value is not finite the rows of the
+// tile are summed key by key instead (attn_slow).
+//
+// Every wait is bounded (tc_common.cuh); one that gives up sets the status word to 2.
+#include <algorithm>
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math_constants.h>
+
+#include "kernels.h"
+#include "mm_terms.cuh"
+#include "pdl.cuh"
+#include "serve_attn.cuh"
+#include "tc_common.cuh"
+
+namespace tlb {
+
+cudaError_t tc_encode_sw128(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides, const uint32_t *box, bool bf16);
+
+namespace sat {
+constexpr int T = 128;
+constexpr int THREADS = 384;            // warp 0 copies, warp 1 issues MMAs, warps 2-3 look through special tiles, 4-7 and 8-11 the streams
+constexpr int HALF_BYTES = T * 128;     // 128 rows of 64 elements
+constexpr float RESCALE_STEP = 8.f;     // in the base-2 domain
+constexpr uint32_t O_COL = 256;         // S / P of stream x at column 128 x, O at 256 + 128 x
+constexpr int SLOW_RING = 16;
+constexpr int OVERHEAD = 1;             // what a row tile costs beside its key tiles, in key tiles
+
+__host__ __device__ constexpr int stages(int hsp, bool share) { return hsp == 128 ? (share ? 2 : 3) : (share ? 4 : 6); }
+__host__ __device__ constexpr int tile_bytes(int hsp) { return T * hsp * 2; }
+__host__ __device__ constexpr int smem_bytes(int hsp, bool share) { return ((share ? 2 : 1) + 2 * stages(hsp, share)) * tile_bytes(hsp); }
+
+struct Params {
+    CUtensorMap q, k, v;
+    ServeAttn a;
+    float scale_log2;
+    int group, tpt, tt;       // heads per KV head; tokens of a row tile; of the row tiles that a unit covers
+    int ctas, min_units;      // a CTA's least share
+    int pool_rows;            // paged: rows of a pool
+    float *partial;           // [CTA][2][rows][2 + hsp]: (m, l) of all rows, then O
+};
+
+// ---- the line of work
+__device__ __forceinline__ int64_t floor_div(int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); }
+// sum of floor((a i + b) / m) for 0 <= i < n, all arguments at least 0
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+    int64_t s = 0;
+    while (n > 0) {
+        s += (n * (n - 1) / 2) * (a / m) + n * (b / m);
+        a %= m;
+        b %= m;
+        const int64_t y = a * n + b;
+        if (y < m) break;
+        n = y / m;
+        b = y % m;
+        const int64_t t = m;
+        m = a;
+        a = t;
+    }
+    return s;
+}
+template <bool PAGED>
+__device__ __forceinline__ int row_tiles(const Params &p, const ServeSeq &s) { return ((PAGED ? p.a.drafts : s.nq) + p.tt - 1) / p.tt; }
+// key tiles of row tile r
+template <bool PAGED>
+__device__ __forceinline__ int key_tiles(const Params &p, const ServeSeq &s, int r) {
+    if (PAGED) return r * p.tt < s.nq ? (int)((s.nk + T - 1) / T) : 0;
+    const int64_t last = min((int64_t)s.nq, (int64_t)(r + 1) * p.tt) - 1 + s.nk - s.nq;   // the last key that its last token sees
+    return last < 0 ? 0 : (int)(last / T) + 1;
+}
+// units of row tiles [0, r)
+template <bool PAGED>
+__device__ __forceinline__ int64_t units_before(const Params &p, const ServeSeq &s, int r) {
+    int64_t u = (int64_t)r * OVERHEAD;
+    if (PAGED) return u + (int64_t)min(r, (s.nq + p.tt - 1) / p.tt) * ((s.nk + T - 1) / T);
+    const int R = row_tiles<false>(p, s);
+    const int full = min(r, R - 1);
+    const int64_t off = s.nk - s.nq;
+    const int first = off < 0 ? (int)min((int64_t)full, -off / p.tt) : 0;   // row tiles that see nothing
+    if (full > first) u += floor_sum(full - first, T, p.tt, off + (int64_t)(first + 1) * p.tt - 1 + T);
+    if (r == R && R > 0) u += key_tiles<false>(p, s, R - 1);
+    return u;
+}
+struct Place {
+    int seq, kvh, r;
+    int64_t off;    // units of this row tile in front of the place
+};
+// The place of unit `at` and the number of all units, by one warp
+template <bool PAGED>
+__device__ __forceinline__ int64_t total_units(const Params &p) {
+    const int lane = threadIdx.x & 31;
+    int64_t u = 0;
+    for (int s = lane; s < p.a.seqs; s += 32) {
+        const ServeSeq q = serve_seq(p.a, s);
+        u += units_before<PAGED>(p, q, row_tiles<PAGED>(p, q)) * p.a.kv_heads;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    return u;
+}
+template <bool PAGED>
+__device__ __forceinline__ Place find_unit(const Params &p, int64_t at) {
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < p.a.seqs; s0 += 32) {
+        int64_t u = 0;
+        if (s0 + lane < p.a.seqs) {
+            const ServeSeq q = serve_seq(p.a, s0 + lane);
+            u = units_before<PAGED>(p, q, row_tiles<PAGED>(p, q)) * p.a.kv_heads;
+        }
+        int64_t upto = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const unsigned in = __ballot_sync(0xffffffffu, at < upto);
+        if (in) {
+            const int l = __ffs(in) - 1;
+            Place w;
+            w.seq = s0 + l;
+            at -= __shfl_sync(0xffffffffu, upto - u, l);
+            const ServeSeq q = serve_seq(p.a, w.seq);
+            const int R = row_tiles<PAGED>(p, q);
+            const int64_t head = units_before<PAGED>(p, q, R);
+            w.kvh = (int)(at / head);
+            at %= head;
+            int lo = 0, hi = R - 1;   // the last row tile that starts at or before `at`
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (units_before<PAGED>(p, q, mid) <= at) lo = mid;
+                else hi = mid - 1;
+            }
+            w.r = lo;
+            w.off = at - units_before<PAGED>(p, q, lo);
+            return w;
+        }
+        at -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return {p.a.seqs, 0, 0, 0};
+}
+__device__ __forceinline__ int64_t share_of(const Params &p, int64_t total) { return max((int64_t)p.min_units, (total + p.ctas - 1) / p.ctas); }
+
+// A stretch of the key tiles of one row tile
+struct Segment {
+    ServeSeq sq;
+    int seq, kvh, r, n, t0, t1;   // key tiles [t0, t1) of n
+    int special;                  // tiles from here on are
+};
+// The stretches of a CTA, the same for all of its warps
+template <bool PAGED>
+struct Walk {
+    Place at;
+    int64_t left;
+    __device__ __forceinline__ bool next(const Params &p, Segment &g) {
+        while (left > 0 && at.seq < p.a.seqs) {
+            const ServeSeq sq = serve_seq(p.a, at.seq);
+            if (at.r >= row_tiles<PAGED>(p, sq)) {
+                at.r = 0;
+                if (row_tiles<PAGED>(p, sq) == 0 || ++at.kvh == p.a.kv_heads) {
+                    at.kvh = 0;
+                    at.seq++;
+                }
+                continue;
+            }
+            const int n = key_tiles<PAGED>(p, sq, at.r);
+            const int64_t take = min(left, n + OVERHEAD - at.off), off = at.off;
+            g.sq = sq;
+            g.seq = at.seq;
+            g.kvh = at.kvh;
+            g.r = at.r;
+            g.n = n;
+            g.t0 = (int)min(off, (int64_t)n);
+            g.t1 = (int)min(off + take, (int64_t)n);
+            // keys that every row of the unit sees: the context, or what its first token sees
+            const int64_t all = PAGED ? sq.nk - sq.nq : max((int64_t)0, (int64_t)at.r * p.tt + sq.nk - sq.nq + 1);
+            g.special = (int)(all / T);
+            left -= take;
+            at.off += take;
+            if (at.off == n + OVERHEAD) {
+                at.off = 0;
+                at.r++;
+            }
+            if (g.t1 > g.t0 || (n == 0 && off == 0)) return true;
+        }
+        return false;
+    }
+};
+
+// What a row sees: keys up to `lim`, or (PAGED) the context and the drafts of `bits`
+struct RowView {
+    int64_t lim;
+    uint64_t bits;
+};
+template <bool PAGED>
+__device__ __forceinline__ bool sees(const RowView &v, int64_t ctx, int64_t key) {
+    if (!PAGED) return key <= v.lim;
+    return key < ctx ? v.lim >= 0 : key - ctx < 64 && ((v.bits >> (key - ctx)) & 1);
+}
+// bit i: the row sees key key0 + i
+template <bool PAGED>
+__device__ __forceinline__ uint32_t seen32(const RowView &v, int64_t ctx, int64_t key0) {
+    if (!PAGED) {
+        const int64_t n = v.lim - key0 + 1;
+        return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << (int)n) - 1u);
+    }
+    if (v.lim < 0) return 0u;
+    const int64_t d = key0 - ctx;   // draft of bit 0
+    if (d <= -32) return 0xffffffffu;
+    if (d < 0) return ((1u << (int)-d) - 1u) | (uint32_t)(v.bits << (int)-d);
+    return d < 64 ? (uint32_t)(v.bits >> (int)d) : 0u;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void fma2(float &x, float &y, uint64_t s, uint64_t c) {
+    uint64_t r = pack2(x, y);
+    asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(r) : "l"(s), "l"(c));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t round2(float a, float b) {
+    if (BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// a += the low half of w, b += the high one, in f32
+template <bool BF16>
+__device__ __forceinline__ void add_halves(uint32_t w, float &a, float &b) {
+    if (BF16) asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.bf16 %0, l, %0;\n\tadd.rn.f32.bf16 %1, h, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(w));
+    else asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.f16 %0, l, %0;\n\tadd.rn.f32.f16 %1, h, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(w));
+}
+__device__ __forceinline__ void ld32(uint32_t taddr, float *x) {
+    uint32_t *r = reinterpret_cast<uint32_t *>(x);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tc::su32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(tc::su32(bar))
+                 : "memory");
+}
+// MN-major, 128-byte swizzle: rows of 64 elements, eight of them to a group of 1 KB; the second 64 columns lie HALF_BYTES further on
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(HALF_BYTES >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// ---- rows of special tiles whose values are not all finite: key by key in f32 (one thread per row)
+template <typename E, bool PAGED>
+__device__ __noinline__ float slow_score(const ServeAttn &a, const ServeSeq &sq, int seq, int kvh, const char *q, int64_t key) {
+    const ServeRow at = serve_kv_row<PAGED>(a, seq, sq, kvh, key);
+    float s = 0.f;
+    if (!at.k) return -CUDART_INF_F;
+    for (int c = 0; c < a.hs / 8; c++) {
+        float x[8], y[8];
+        serve_unpack<E>(*reinterpret_cast<const uint4 *>(q + c * 16), x);
+        serve_unpack<E>(*reinterpret_cast<const uint4 *>(at.k + c * 16), y);
+#pragma unroll
+        for (int e = 0; e < 8; e++) s = fmaf(x[e], y[e], s);
+    }
+    return s;
+}
+template <typename E, bool PAGED>
+__device__ __noinline__ void slow_stats(const Params &p, const Segment &g, const RowView &v, const char *q, float &m, float &l) {
+    const int64_t ctx = g.sq.nk - g.sq.nq, k1 = min(g.sq.nk, (int64_t)g.t1 * T);
+    m = -CUDART_INF_F;
+    l = 0.f;
+    for (int64_t key = (int64_t)g.t0 * T; key < k1; key++)
+        if (sees<PAGED>(v, ctx, key)) m = fmaxf(m, slow_score<E, PAGED>(p.a, g.sq, g.seq, g.kvh, q, key) * p.scale_log2);
+    const float ref = m == -CUDART_INF_F ? 0.f : m;
+    for (int64_t key = (int64_t)g.t0 * T; key < k1; key++)
+        if (sees<PAGED>(v, ctx, key)) l += ex2(slow_score<E, PAGED>(p.a, g.sq, g.seq, g.kvh, q, key) * p.scale_log2 - ref);
+    m = ref;
+}
+// columns [c0, c0 + 32) of the unnormalised result
+template <typename E, bool PAGED>
+__device__ __noinline__ void slow_columns(const Params &p, const Segment &g, const RowView &v, const char *q, float m, int c0, float *o) {
+    const int64_t ctx = g.sq.nk - g.sq.nq, k1 = min(g.sq.nk, (int64_t)g.t1 * T);
+    for (int i = 0; i < 32; i++) o[i] = 0.f;
+    for (int64_t key = (int64_t)g.t0 * T; key < k1; key++) {
+        if (!sees<PAGED>(v, ctx, key)) continue;
+        const ServeRow at = serve_kv_row<PAGED>(p.a, g.seq, g.sq, g.kvh, key);
+        if (!at.v) continue;
+        const float w = ex2(slow_score<E, PAGED>(p.a, g.sq, g.seq, g.kvh, q, key) * p.scale_log2 - m);
+        for (int c = 0; c < 4; c++) {
+            if (c0 + c * 8 >= p.a.hs) break;
+            float y[8];
+            serve_unpack<E>(*reinterpret_cast<const uint4 *>(at.v + (c0 + c * 8) * 2), y);
+            for (int e = 0; e < 8; e++) o[c * 8 + e] = fmaf(w, y[e], o[c * 8 + e]);
+        }
+    }
+}
+}  // namespace sat
+
+template <int HSP, bool BF16, bool PAGED, bool SHARE>
+__global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_constant__ sat::Params p) {
+    using namespace tc;
+    using namespace sat;
+    using E = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    constexpr int NS = stages(HSP, SHARE), TILE = tile_bytes(HSP), HALVES = HSP / 64, NQ = SHARE ? 2 : 1;
+    constexpr uint32_t FMT = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(T >> 4) << 24);
+    constexpr uint32_t IDESC_QK = FMT | ((uint32_t)(T >> 3) << 17), IDESC_PV = FMT | (1u << 16) | ((uint32_t)(HSP >> 3) << 17);
+    extern __shared__ __align__(1024) uint8_t smem[];   // behind 3 KB of the arrays below, so that three stages fill the 227 KB to the byte
+    uint8_t *qs = smem, *ks = qs + NQ * TILE, *vs = ks + NS * TILE;
+    __shared__ uint64_t bar_q, bar_qfree, bar_k[NS], bar_kfree[NS], bar_v[NS], bar_vfree[NS], bar_fix[NS], bar_s[2], bar_p[2], bar_o[2], bar_od;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int s_fail;
+    __shared__ volatile int slow_ring[SLOW_RING];   // segment + 1 of those whose special tiles hold values that are not finite
+    __shared__ Walk<PAGED> walks[sat::THREADS / 32];   // in shared memory between segments: the streams' registers are full of scores
+    __shared__ float pair_ml[2][T][2];
+    volatile int *fail = &s_fail;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    griddep_launch();
+    if (tid == 0) {
+        mbar_init(&bar_q, 1);
+        mbar_init(&bar_qfree, 1);
+        for (int i = 0; i < NS; i++) {
+            mbar_init(&bar_k[i], 1);
+            mbar_init(&bar_kfree[i], 1);
+            mbar_init(&bar_v[i], 1);
+            mbar_init(&bar_vfree[i], 1);
+            mbar_init(&bar_fix[i], 2);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bar_s[i], 1);
+            mbar_init(&bar_p[i], 4);
+            mbar_init(&bar_o[i], 1);
+        }
+        mbar_init(&bar_od, 8);
+        s_fail = 0;
+        for (int i = 0; i < SLOW_RING; i++) slow_ring[i] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc(&tmem_base_s, 512);
+    griddep_wait();
+    if (warp == 3) {
+        const int64_t total = total_units<PAGED>(p), share = share_of(p, total), a0 = share * blockIdx.x;
+        const int64_t mine = min(share, total - a0);
+        const Place w = mine > 0 ? find_unit<PAGED>(p, a0) : Place{p.a.seqs, 0, 0, 0};
+        if (lane < sat::THREADS / 32) {
+            walks[lane].at = w;
+            walks[lane].left = mine;
+        }
+    }
+    if (warp == 2 && blockIdx.x == 0 && p.a.err) {
+        for (int s = lane; s < p.a.seqs; s += 32)
+            if (!serve_seq(p.a, s).ok) report_error(p.a.err, TLB_ERR_INDEX);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
+    Segment g;
+    auto next = [&]() {
+        Walk<PAGED> w = walks[warp];
+        __syncwarp();
+        const bool more = w.next(p, g);
+        if (lane == 0) walks[warp] = w;
+        __syncwarp();
+        return more;
+    };
+
+    if (warp == 0) {
+        // ---- copies. The keys of a segment's first tiles are on their way before its queries, whose room the segment in front still uses.
+        int tile = 0, seg = 0;
+        while (next()) {
+            if (g.t1 == g.t0) continue;   // a row tile that sees nothing has no part in the pipeline's counts
+            bool have_q = false;
+            auto load_q = [&]() {
+                if (lane == 0) {
+                    mbar_wait_nap(&bar_qfree, (uint32_t)(seg + 1) & 1u, fail, 32);
+                    mbar_expect_tx(&bar_q, (uint32_t)(NQ * HALVES * 128 * p.group * p.tpt));
+                    for (int x = 0; x < NQ; x++)
+                        for (int h = 0; h < HALVES; h++)
+                            tma_3d(qs + x * TILE + h * HALF_BYTES, &p.q, h * 64, g.kvh * p.group, (int)(g.sq.q0 + (int64_t)g.r * p.tt + x * p.tpt), &bar_q);
+                }
+                have_q = true;
+            };
+            for (int j = g.t0; j < g.t1; j++, tile++) {
+                if (!have_q && (j - g.t0 >= NS || __any_sync(0xffffffffu, mbar_test(su32(&bar_qfree), (uint32_t)(seg + 1) & 1u)))) load_q();
+                const int s = tile % NS;
+                const uint32_t free_parity = (uint32_t)(tile / NS + 1) & 1u;
+                if (!PAGED) {
+                    if (lane == 0) {
+                        const int z = (int)(g.sq.k0 + (int64_t)j * T);
+                        mbar_wait_nap(&bar_kfree[s], free_parity, fail, 32);
+                        mbar_expect_tx(&bar_k[s], TILE);
+                        for (int h = 0; h < HALVES; h++) tma_3d(ks + s * TILE + h * HALF_BYTES, &p.k, h * 64, g.kvh, z, &bar_k[s]);
+                        mbar_wait_nap(&bar_vfree[s], free_parity, fail, 32);
+                        mbar_expect_tx(&bar_v[s], TILE);
+                        for (int h = 0; h < HALVES; h++) tma_3d(vs + s * TILE + h * HALF_BYTES, &p.v, h * 64, g.kvh, z, &bar_v[s]);
+                    }
+                } else {
+                    // a box per page and 64 columns, a lane each; pages that are not needed and bad ids lie past the pool: zeros
+                    const int rows = min(p.a.block_size, T), boxes = T / rows;   // 1 to 16 pages
+                    int row = p.pool_rows;
+                    if (lane < boxes) {
+                        const int64_t key = (int64_t)j * T + lane * rows;
+                        if (key < g.sq.nk) {
+                            const int32_t blk = p.a.tables[(int64_t)g.seq * p.a.max_blocks + key / p.a.block_size];
+                            if (blk >= 0 && blk < p.a.pool_blocks) row = (blk * p.a.kv_heads + g.kvh) * p.a.block_size + (int)(key % p.a.block_size);
+                            else if (p.a.err) report_error(p.a.err, TLB_ERR_INDEX);
+                        }
+                    }
+                    row = __shfl_sync(0xffffffffu, row, lane % boxes);
+                    const int h = lane / boxes, dst = h * HALF_BYTES + lane % boxes * rows * 128;
+                    mbar_wait_nap(&bar_kfree[s], free_parity, fail, 32);
+                    if (lane == 0) mbar_expect_tx(&bar_k[s], TILE);
+                    __syncwarp();
+                    if (h < HALVES) tma_2d(ks + s * TILE + dst, &p.k, h * 64, row, &bar_k[s]);
+                    mbar_wait_nap(&bar_vfree[s], free_parity, fail, 32);
+                    if (lane == 0) mbar_expect_tx(&bar_v[s], TILE);
+                    __syncwarp();
+                    if (h < HALVES) tma_2d(vs + s * TILE + dst, &p.v, h * 64, row, &bar_v[s]);
+                }
+                if (__any_sync(0xffffffffu, *fail)) break;
+            }
+            if (__any_sync(0xffffffffu, *fail)) break;
+            if (!have_q) load_q();
+            __syncwarp();
+            seg++;
+        }
+        // only after a wait has given up: this CTA's copies are over before its shared memory is
+        if (*fail && lane == 0) {
+            mbar_wait_limit(&bar_q, 0, 1u << 12);
+            for (int i = 0; i < NS; i++) {
+                mbar_wait_limit(&bar_k[i], 0, 1u << 10);
+                mbar_wait_limit(&bar_k[i], 1, 1u << 10);
+                mbar_wait_limit(&bar_v[i], 0, 1u << 10);
+                mbar_wait_limit(&bar_v[i], 1, 1u << 10);
+            }
+        }
+    } else if (warp == 1) {
+        // ---- MMA issue: step i is stream i & 1; S of step i + 2 follows O of step i, which has read the P that it overwrites
+        const bool leader = elect_one();
+        int tile = 0, seg = 0;
+        uint32_t n_p[2] = {0, 0};
+        while (next()) {
+            const int n = g.t1 - g.t0, steps = SHARE ? 2 * n : n;
+            if (n == 0) continue;
+            auto issue_s = [&](int i) {
+                const int x = i & 1, k = tile + (SHARE ? i >> 1 : i), s = k % NS;
+                if (!SHARE || x == 0) mbar_wait_nap(&bar_k[s], (uint32_t)(k / NS) & 1u, fail, 0);
+                tc_fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++) {
+                        const uint64_t qd = plain::desc_sw128(su32(qs + (SHARE ? x * TILE : 0) + h * HALF_BYTES)), kd = plain::desc_sw128(su32(ks + s * TILE + h * HALF_BYTES));
+#pragma unroll
+                        for (int e = 0; e < 4; e++) umma_f16(tmem + (uint32_t)(x * T), qd + 2 * e, kd + 2 * e, IDESC_QK, (h | e) ? 1u : 0u);
+                    }
+                    umma_commit(&bar_s[x]);
+                    if (!SHARE || x == 1) umma_commit(&bar_kfree[s]);
+                    if (i == steps - 1) umma_commit(&bar_qfree);
+                }
+                __syncwarp();
+            };
+            mbar_wait_nap(&bar_q, (uint32_t)seg & 1u, fail, 0);
+            issue_s(0);
+            if (steps > 1) issue_s(1);
+            for (int i = 0; i < steps; i++) {
+                const int x = i & 1, j = SHARE ? i >> 1 : i, k = tile + j, s = k % NS;
+                if (!SHARE || x == 0) mbar_wait_nap(&bar_fix[s], (uint32_t)(k / NS) & 1u, fail, 0);
+                mbar_wait_nap(&bar_p[x], (n_p[x]++) & 1u, fail, 0);
+                if (i == 0 && seg > 0) mbar_wait_nap(&bar_od, (uint32_t)(seg - 1) & 1u, fail, 0);
+                tc_fence_after();
+                if (leader) {
+                    const uint64_t vd = desc_mn(su32(vs + s * TILE));
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        umma_f16_ta(tmem + O_COL + (uint32_t)(x * T), tmem + (uint32_t)(x * T + e * 8), vd + (uint64_t)(e * 128), IDESC_PV, (i > 1 || e) ? 1u : 0u);
+                    umma_commit(&bar_o[x]);
+                    if (!SHARE || x == 1) umma_commit(&bar_vfree[s]);
+                }
+                __syncwarp();
+                if (i + 2 < steps) issue_s(i + 2);
+            }
+            tile += n;
+            seg++;
+        }
+    } else if (warp < 4) {
+        // ---- every tile of values passes here, in order, on its way to the MMAs. Special ones: rows behind the end become zero, the others are
+        // looked through
+        int tile = 0, seg = 0;
+        while (next()) {
+            if (g.t1 == g.t0) continue;
+            for (int j = g.t0; j < g.t1; j++, tile++) {
+                const int s = tile % NS;
+                mbar_wait_nap(&bar_v[s], (uint32_t)(tile / NS) & 1u, fail, 0);
+                if (j >= g.special) {
+                    const int live = (int)min((int64_t)T, g.sq.nk - (int64_t)j * T);
+                    uint4 *v = reinterpret_cast<uint4 *>(vs + s * TILE);
+                    constexpr uint32_t EXP = BF16 ? 0x7f807f80u : 0x7c007c00u;
+                    uint32_t odd = 0;
+#pragma unroll 8
+                    for (int i = tid - 64; i < TILE / 16; i += 64) {
+                        if (((i >> 3) & (T - 1)) >= live) {
+                            v[i] = make_uint4(0, 0, 0, 0);
+                        } else {
+                            const uint4 w = v[i];
+                            odd |= __vcmpeq2(w.x & EXP, EXP) | __vcmpeq2(w.y & EXP, EXP) | __vcmpeq2(w.z & EXP, EXP) | __vcmpeq2(w.w & EXP, EXP);
+                        }
+                    }
+                    if (odd) slow_ring[seg % SLOW_RING] = seg + 1;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_fix[s]);
+            }
+            seg++;
+        }
+    } else {
+        // ---- the streams
+        const int x = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+        const uint32_t s_at = lanes + (uint32_t)(x * T), o_at = lanes + O_COL + (uint32_t)(x * T);
+        int seg = 0;
+        uint32_t done[2] = {0, 0};   // tiles of either stream so far
+        while (next()) {
+            const int64_t ctx = g.sq.nk - g.sq.nq;
+            const int token = g.r * p.tt + (SHARE ? x * p.tpt : 0) + row / p.group, head = g.kvh * p.group + row % p.group;
+            const bool live_row = row < p.tpt * p.group && token < (PAGED ? p.a.drafts : g.sq.nq);
+            RowView view;
+            view.bits = 0;
+            view.lim = live_row && token < g.sq.nq ? ctx + token : -1;
+            if (PAGED && view.lim >= 0) view.bits = serve_ancestors(p.a, g.seq, token);
+            const int n = g.t1 - g.t0;
+            const int mine = SHARE ? n : (n + 1 - x) / 2, other = SHARE ? n : (n + x) / 2;
+            float m_ref = 0.f, l = 0.f;
+            bool have_ref = false;
+            for (int i = 0; i < mine; i++) {
+                const int j = g.t0 + (SHARE ? i : 2 * i + x);
+                mbar_wait_nap(&bar_s[x], (done[x] + i) & 1u, fail, 0);
+                tc_fence_after();
+                float y[T];
+#pragma unroll
+                for (int c = 0; c < 4; c++) ld32(s_at + 32 * c, y + 32 * c);
+                tmem_ld_wait();
+                if (j >= g.special) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const uint32_t seen = seen32<PAGED>(view, ctx, (int64_t)j * T + 32 * c);
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (!((seen >> e) & 1u)) y[32 * c + e] = -CUDART_INF_F;
+                    }
+                }
+                float mx = y[0];
+#pragma unroll
+                for (int e = 1; e < T; e++) mx = fmaxf(mx, y[e]);
+                mx *= p.scale_log2;
+                float alpha = 1.f;
+                if (!have_ref) {
+                    if (mx != -CUDART_INF_F) {
+                        m_ref = mx;
+                        have_ref = true;   // nothing has been added up for this row yet
+                    }
+                } else if (mx > m_ref + RESCALE_STEP) {
+                    alpha = ex2(m_ref - mx);
+                    m_ref = mx;
+                }
+                if (__any_sync(0xffffffffu, alpha != 1.f)) {   // never on a segment's first tile
+                    mbar_wait_nap(&bar_o[x], (done[x] + i - 1) & 1u, fail, 0);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HSP / 32; c++) {
+                        float o[32];
+                        ld32(o_at + 32 * c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] *= alpha;
+                        st32(o_at + 32 * c, reinterpret_cast<const uint32_t *>(o));
+                    }
+                    l *= alpha;
+                }
+                const uint64_t sc = pack2(p.scale_log2, p.scale_log2), ref = pack2(-m_ref, -m_ref);
+                float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        float a = y[64 * c + 2 * e], b = y[64 * c + 2 * e + 1];
+                        fma2(a, b, sc, ref);
+                        w[e] = round2<BF16>(ex2(a), ex2(b));
+                        add_halves<BF16>(w[e], sum0, sum1);
+                    }
+                    st32(s_at + 32 * c, w);
+                }
+                l += sum0 + sum1;
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_p[x]);
+            }
+            done[x] += mine;
+            done[x ^ 1] += other;
+            // ---- the segment's result: O / l, or (m, l, O) where the row tile was cut
+            if (mine > 0) mbar_wait_nap(&bar_o[x], (done[x] - 1) & 1u, fail, 0);
+            if (!SHARE && other > 0) mbar_wait_nap(&bar_o[x ^ 1], (done[x ^ 1] - 1) & 1u, fail, 0);
+            tc_fence_after();
+            const bool slow = n > 0 && slow_ring[seg % SLOW_RING] == seg + 1;
+            const char *q = (const char *)p.a.q + (g.sq.q0 + token) * p.a.q_stride + (int64_t)head * p.a.hs * 2;
+            float f_mine = 1.f, f_other = 0.f;
+            if (slow) {
+                if (view.lim >= 0) slow_stats<E, PAGED>(p, g, view, q, m_ref, l);
+                __syncwarp();
+            } else if (!SHARE) {
+                pair_ml[x][row][0] = have_ref ? m_ref : -CUDART_INF_F;
+                pair_ml[x][row][1] = l;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const float m2 = pair_ml[x ^ 1][row][0], l2 = pair_ml[x ^ 1][row][1], m1 = have_ref ? m_ref : -CUDART_INF_F;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                m_ref = fmaxf(m1, m2);
+                if (m_ref == -CUDART_INF_F) m_ref = 0.f;
+                f_mine = ex2(m1 - m_ref);
+                f_other = ex2(m2 - m_ref);
+                l = l * f_mine + l2 * f_other;
+            }
+            if (view.lim < 0) l = 0.f;   // a row that sees nothing, or no token's
+            const bool whole = g.t0 == 0 && g.t1 == g.n;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            float *part = whole ? nullptr : p.partial + ((size_t)blockIdx.x * 2 + (g.t0 > 0 ? 0 : 1)) * (NQ * T) * (2 + HSP);
+            const int prow = (SHARE ? x * T : 0) + row;
+            if (!whole && (SHARE || x == 0)) {
+                part[prow * 2] = m_ref;
+                part[prow * 2 + 1] = l;
+            }
+            // SHARE: a thread writes its row; else the streams take half of the columns each
+            constexpr int COLS = SHARE ? HSP : HSP / 2;
+            const int c_first = SHARE ? 0 : x * COLS;
+#pragma unroll 1
+            for (int c0 = c_first; c0 < c_first + COLS; c0 += 32) {
+                float o[32];
+                __syncwarp();
+                if (slow) {
+                    if (view.lim >= 0) slow_columns<E, PAGED>(p, g, view, q, m_ref, c0, o);
+                    __syncwarp();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0.f;
+                    if (mine > 0) {
+                        ld32(o_at + c0, o);
+                        tmem_ld_wait();
+                    }
+                    if (!SHARE) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] *= f_mine;
+                        if (other > 0) {
+                            float o2[32];
+                            ld32(lanes + O_COL + (uint32_t)((x ^ 1) * T) + c0, o2);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] = fmaf(o2[e], f_other, o[e]);
+                        }
+                    }
+                }
+                if (view.lim < 0) {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0.f;
+                }
+                if (whole) {
+                    if (live_row) {
+                        char *dst = (char *)p.a.out + (g.sq.q0 + token) * p.a.out_stride + (int64_t)head * p.a.hs * 2;
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (c0 + 8 * e < p.a.hs)
+                                *reinterpret_cast<uint4 *>(dst + (c0 + 8 * e) * 2) =
+                                    make_uint4(round2<BF16>(o[8 * e] * inv, o[8 * e + 1] * inv), round2<BF16>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                               round2<BF16>(o[8 * e + 4] * inv, o[8 * e + 5] * inv), round2<BF16>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+                    }
+                } else if (live_row) {
+                    float4 *dst = reinterpret_cast<float4 *>(part + NQ * T * 2 + (size_t)prow * HSP + c0);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (n == 0) continue;
+            if (lane == 0) mbar_arrive(&bar_od);
+            seg++;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem, 512);
+    if (tid == 0 && s_fail && p.a.err) report_error(p.a.err, 2);
+}
+
+// Row tiles that were cut: CTA (c, rows) adds up the parts of the one that begins in stretch c of the line and reaches over its end.
+template <int HSP, bool BF16, bool PAGED, bool SHARE>
+__global__ void __launch_bounds__(128) k_serve_join(const __grid_constant__ sat::Params p) {
+    using namespace sat;
+    constexpr int NQ = SHARE ? 2 : 1, ROWS = NQ * T, SLOT = ROWS * (2 + HSP);
+    griddep_launch();
+    griddep_wait();
+    __shared__ Place at_s;
+    __shared__ int64_t share_s;
+    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 0) {
+        const int64_t total = total_units<PAGED>(p), share = share_of(p, total), end = share * (c + 1);
+        const Place w = end < total ? find_unit<PAGED>(p, end) : Place{p.a.seqs, 0, 0, 0};
+        if (lane == 0) {
+            at_s = w;
+            share_s = share;
+        }
+    }
+    __syncthreads();
+    const Place w = at_s;
+    if (w.seq >= p.a.seqs || w.off == 0 || w.off > share_s) return;   // nothing begins here, or in a stretch in front
+    const ServeSeq sq = serve_seq(p.a, w.seq);
+    const int n = key_tiles<PAGED>(p, sq, w.r);
+    if (w.off >= n) return;   // all of its key tiles lie in this stretch
+    const int parts = 1 + (int)((n - w.off + share_s - 1) / share_s);
+    for (int row = blockIdx.y * 8 + warp; row < (int)blockIdx.y * 8 + 8; row += 4) {
+        const int x = row / T, rr = row % T;
+        const int token = w.r * p.tt + x * p.tpt + rr / p.group, head = w.kvh * p.group + rr % p.group;
+        if (rr >= p.tpt * p.group || token >= (PAGED ? p.a.drafts : sq.nq)) continue;
+        float m = -CUDART_INF_F;
+        auto slot = [&](int i) { return p.partial + ((size_t)(c + i) * 2 + (i ? 0 : 1)) * SLOT; };
+        for (int i = lane; i < parts; i += 32) m = fmaxf(m, slot(i)[row * 2 + 1] == 0.f ? -CUDART_INF_F : slot(i)[row * 2]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (m == -CUDART_INF_F) m = 0.f;
+        float l = 0.f, o[HSP / 32];
+#pragma unroll
+        for (int e = 0; e < HSP / 32; e++) o[e] = 0.f;
+        for (int i = 0; i < parts; i++) {
+            const float *s = slot(i), li = s[row * 2 + 1];
+            if (li == 0.f) continue;   // a part in which the row sees nothing
+            const float f = ex2(s[row * 2] - m);
+            l = fmaf(li, f, l);
+#pragma unroll
+            for (int e = 0; e < HSP / 32; e++) o[e] = fmaf(s[ROWS * 2 + row * HSP + lane * (HSP / 32) + e], f, o[e]);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        using E = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+        E *dst = reinterpret_cast<E *>((char *)p.a.out + (sq.q0 + token) * p.a.out_stride) + (int64_t)head * p.a.hs;
+#pragma unroll
+        for (int e = 0; e < HSP / 32; e++)
+            if (lane * (HSP / 32) + e < p.a.hs) dst[lane * (HSP / 32) + e] = serve_round<E>(o[e] * inv);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+bool serve_attn_tc_supported(const ServeAttn &a) {
+    if (!tc_available() || a.hs > 128 || a.heads / a.kv_heads > sat::T) return false;
+    if (a.paged) return a.block_size >= 8 && a.pool_blocks > 0 && a.pool_blocks * a.kv_heads * a.block_size < 0x7fffffff;
+    return a.kv_rows > 0;
+}
+// A pair of row tiles per unit where sequences fill them on average.
+static bool sat_share(const ServeAttn &a) { return !a.paged && a.q_rows * (a.heads / a.kv_heads) > (int64_t)a.seqs * sat::T; }
+static int sat_ctas(const ServeAttn &a, int sm_count) {
+    const bool share = sat_share(a);
+    const int64_t tt = (int64_t)(sat::T / (a.heads / a.kv_heads)) * (share ? 2 : 1);
+    const int64_t tiles = a.paged ? (a.drafts + tt - 1) / tt * a.seqs : a.q_rows / tt + a.seqs;
+    const int64_t keys = a.paged ? ((int64_t)a.max_blocks * a.block_size + sat::T - 1) / sat::T : (a.kv_rows + sat::T - 1) / sat::T;
+    const double units = (double)tiles * a.kv_heads * (double)(keys + sat::OVERHEAD);
+    return units / 2 < sm_count ? std::max(1, (int)(units / 2 + 1)) : sm_count;
+}
+uint64_t serve_attn_tc_scratch_bytes(const ServeAttn &a, int sm_count) {
+    return (uint64_t)sat_ctas(a, sm_count) * 2 * (sat_share(a) ? 2 : 1) * sat::T * (2 + (a.hs <= 64 ? 64 : 128)) * 4;
+}
+template <int HSP, bool BF16, bool PAGED, bool SHARE>
+static cudaError_t sat_launch(const sat::Params &p, int ctas, cudaStream_t st) {
+    cudaError_t e = launch_pdl(k_serve_attn_tc<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas), dim3(sat::THREADS), sat::smem_bytes(HSP, SHARE), st, p);
+    if (e == cudaSuccess && ctas > 1) e = launch_pdl(k_serve_join<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas - 1, (SHARE ? 2 : 1) * sat::T / 8), dim3(128), 0, st, p);
+    return e;
+}
+template <int HSP, bool BF16, bool PAGED, bool SHARE>
+static void sat_configure() {
+    cudaFuncSetAttribute(k_serve_attn_tc<HSP, BF16, PAGED, SHARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, sat::smem_bytes(HSP, SHARE));
+}
+void serve_attn_tc_configure() {
+    sat_configure<64, false, false, false>();
+    sat_configure<64, false, false, true>();
+    sat_configure<64, true, false, false>();
+    sat_configure<64, true, false, true>();
+    sat_configure<128, false, false, false>();
+    sat_configure<128, false, false, true>();
+    sat_configure<128, true, false, false>();
+    sat_configure<128, true, false, true>();
+    sat_configure<64, false, true, false>();
+    sat_configure<128, false, true, false>();
+}
+cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count, cudaStream_t st) {
+    using namespace sat;
+    Params p{};
+    p.a = a;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.group = a.heads / a.kv_heads;
+    p.tpt = T / p.group;
+    const bool share = sat_share(a);
+    p.tt = p.tpt * (share ? 2 : 1);
+    p.min_units = 1 + OVERHEAD;
+    p.partial = (float *)scratch;
+    const uint64_t hs = (uint64_t)a.hs;
+    cudaError_t e;
+    {
+        const uint64_t dims[3] = {hs, (uint64_t)a.heads, (uint64_t)a.q_rows}, strides[2] = {hs * 2, (uint64_t)a.q_stride};
+        const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)p.tpt};
+        e = tc_encode_sw128(&p.q, a.q, 3, dims, strides, box, a.bf16);
+    }
+    for (int i = 0; i < 2 && e == cudaSuccess; i++) {
+        if (a.paged) {
+            p.pool_rows = (int)(a.pool_blocks * a.kv_heads * a.block_size);
+            const uint64_t dims[2] = {hs, (uint64_t)p.pool_rows}, strides[1] = {hs * 2};
+            const uint32_t box[2] = {64, (uint32_t)std::min(a.block_size, T)};
+            e = tc_encode_sw128(i ? &p.v : &p.k, i ? a.v : a.k, 2, dims, strides, box, false);
+        } else {
+            const uint64_t dims[3] = {hs, (uint64_t)a.kv_heads, (uint64_t)a.kv_rows}, strides[2] = {hs * 2, (uint64_t)(i ? a.v_stride : a.k_stride)};
+            const uint32_t box[3] = {64, 1, T};
+            e = tc_encode_sw128(i ? &p.v : &p.k, i ? a.v : a.k, 3, dims, strides, box, a.bf16);
+        }
+    }
+    if (e != cudaSuccess) return e;
+    const int ctas = p.ctas = sat_ctas(a, sm_count);
+    if (a.paged) return a.hs <= 64 ? sat_launch<64, false, true, false>(p, ctas, st) : sat_launch<128, false, true, false>(p, ctas, st);
+    if (a.hs <= 64) {
+        if (a.bf16) return share ? sat_launch<64, true, false, true>(p, ctas, st) : sat_launch<64, true, false, false>(p, ctas, st);
+        return share ? sat_launch<64, false, false, true>(p, ctas, st) : sat_launch<64, false, false, false>(p, ctas, st);
+    }
+    if (a.bf16) return share ? sat_launch<128, true, false, true>(p, ctas, st) : sat_launch<128, true, false, false>(p, ctas, st);
+    return share ? sat_launch<128, false, false, true>(p, ctas, st) : sat_launch<128, false, false, false>(p, ctas, st);
+}
+
+}  // namespace tlb

@@ -339,6 +339,10 @@ constexpr int TREE_MAX_DRAFTS = 64;   // a token's ancestors are a 64-bit mask
 const char *serve_attn_refusal(const ServeAttn &a);   // why the shapes are not supported, or null
 uint64_t serve_attn_scratch_bytes(const ServeAttn &a, int sm_count);
 cudaError_t launch_serve_attn(const ServeAttn &a, void *scratch, int sm_count, cudaStream_t st);
+bool serve_attn_tc_supported(const ServeAttn &a);
+uint64_t serve_attn_tc_scratch_bytes(const ServeAttn &a, int sm_count);
+cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count, cudaStream_t st);
+void serve_attn_tc_configure();
 // The accepted drafts of every sequence (their places among the drafts, rising) to positions context, context + 1, ... in the pools of all layers
 struct CacheKeep {
     void *kpool, *vpool;           // of the first layer
