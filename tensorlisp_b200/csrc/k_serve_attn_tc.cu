@@ -46,7 +46,8 @@ constexpr int HALF_BYTES = T * 128;     // 128 rows of 64 elements
 constexpr float RESCALE_STEP = 8.f;     // in the base-2 domain
 constexpr uint32_t O_COL = 256;         // S / P of stream x at column 128 x, O at 256 + 128 x
 constexpr int SLOW_RING = 16;
-constexpr int OVERHEAD = 1;             // what a row tile costs beside its key tiles, in key tiles
+constexpr int REGS_ROLES = 88, REGS_STREAMS = 200;   // registers of a thread (setmaxnreg): the streams hold a row of 128 scores
+constexpr int OVERHEAD = 2;             // what a row tile costs beside its key tiles, in key tiles
 
 __host__ __device__ constexpr int stages(int hsp, bool share) { return hsp == 128 ? (share ? 2 : 3) : (share ? 4 : 6); }
 __host__ __device__ constexpr int tile_bytes(int hsp) { return T * hsp * 2; }
@@ -59,23 +60,23 @@ struct Params {
     int group, tpt, tt;       // heads per KV head; tokens of a row tile; of the row tiles that a unit covers
     int ctas, min_units;      // a CTA's least share
     int pool_rows;            // paged: rows of a pool
-    float *partial;           // [CTA][2][rows][2 + hsp]: (m, l) of all rows, then O
+    float *partial;           // [CTA][2]: (m, l) of the rows, then O as [hsp / 4][rows][4], which the writers' lanes (rows) fill side by side
 };
 
 // ---- the line of work
-__device__ __forceinline__ int64_t floor_div(int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); }
-// sum of floor((a i + b) / m) for 0 <= i < n, all arguments at least 0
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+// sum of floor((a i + b) / m) for 0 <= i < n; a n + b below 2^32
+__device__ __forceinline__ int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
     int64_t s = 0;
     while (n > 0) {
-        s += (n * (n - 1) / 2) * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
-        const int64_t y = a * n + b;
+        const uint32_t qa = a / m, qb = b / m;
+        s += (int64_t)n * (n - 1) / 2 * qa + (int64_t)n * qb;
+        a -= qa * m;
+        b -= qb * m;
+        const uint32_t y = a * n + b;   // what is left of it, turned on its side
         if (y < m) break;
         n = y / m;
-        b = y % m;
-        const int64_t t = m;
+        b = y - n * m;
+        const uint32_t t = m;
         m = a;
         a = t;
     }
@@ -99,7 +100,10 @@ __device__ __forceinline__ int64_t units_before(const Params &p, const ServeSeq 
     const int full = min(r, R - 1);
     const int64_t off = s.nk - s.nq;
     const int first = off < 0 ? (int)min((int64_t)full, -off / p.tt) : 0;   // row tiles that see nothing
-    if (full > first) u += floor_sum(full - first, T, p.tt, off + (int64_t)(first + 1) * p.tt - 1 + T);
+    if (full > first) {   // floor((off + (i + 1) tt - 1) / T) + 1 of the tiles in between; whole key tiles of off go in front
+        const int64_t b = off + (int64_t)(first + 1) * p.tt - 1 + T;
+        u += (int64_t)(full - first) * (b / T) + floor_sum((uint32_t)(full - first), T, (uint32_t)p.tt, (uint32_t)(b % T));
+    }
     if (r == R && R > 0) u += key_tiles<false>(p, s, R - 1);
     return u;
 }
@@ -107,28 +111,28 @@ struct Place {
     int seq, kvh, r;
     int64_t off;    // units of this row tile in front of the place
 };
-// The place of unit `at` and the number of all units, by one warp
+// By one warp: the number of all units, and the place of one
 template <bool PAGED>
-__device__ __forceinline__ int64_t total_units(const Params &p) {
+__device__ __forceinline__ int64_t seq_units(const Params &p, int s) {
+    if (s >= p.a.seqs) return 0;
+    const ServeSeq q = serve_seq(p.a, s);
+    return units_before<PAGED>(p, q, row_tiles<PAGED>(p, q)) * p.a.kv_heads;
+}
+// first: the units of sequence `lane`, which find_unit begins with
+template <bool PAGED>
+__device__ __forceinline__ int64_t total_units(const Params &p, int64_t &first) {
     const int lane = threadIdx.x & 31;
-    int64_t u = 0;
-    for (int s = lane; s < p.a.seqs; s += 32) {
-        const ServeSeq q = serve_seq(p.a, s);
-        u += units_before<PAGED>(p, q, row_tiles<PAGED>(p, q)) * p.a.kv_heads;
-    }
+    int64_t u = first = seq_units<PAGED>(p, lane);
+    for (int s = lane + 32; s < p.a.seqs; s += 32) u += seq_units<PAGED>(p, s);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
     return u;
 }
 template <bool PAGED>
-__device__ __forceinline__ Place find_unit(const Params &p, int64_t at) {
+__device__ __forceinline__ Place find_unit(const Params &p, int64_t at, int64_t first) {
     const int lane = threadIdx.x & 31;
     for (int s0 = 0; s0 < p.a.seqs; s0 += 32) {
-        int64_t u = 0;
-        if (s0 + lane < p.a.seqs) {
-            const ServeSeq q = serve_seq(p.a, s0 + lane);
-            u = units_before<PAGED>(p, q, row_tiles<PAGED>(p, q)) * p.a.kv_heads;
-        }
+        const int64_t u = s0 ? seq_units<PAGED>(p, s0 + lane) : first;
         int64_t upto = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -141,19 +145,23 @@ __device__ __forceinline__ Place find_unit(const Params &p, int64_t at) {
             Place w;
             w.seq = s0 + l;
             at -= __shfl_sync(0xffffffffu, upto - u, l);
-            const ServeSeq q = serve_seq(p.a, w.seq);
-            const int R = row_tiles<PAGED>(p, q);
-            const int64_t head = units_before<PAGED>(p, q, R);
+            const int64_t head = __shfl_sync(0xffffffffu, u, l) / p.a.kv_heads;
             w.kvh = (int)(at / head);
-            at %= head;
-            int lo = 0, hi = R - 1;   // the last row tile that starts at or before `at`
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) / 2;
-                if (units_before<PAGED>(p, q, mid) <= at) lo = mid;
-                else hi = mid - 1;
+            at -= w.kvh * head;
+            // the last row tile that starts at or before `at`: 32 places at a time
+            const ServeSeq q = serve_seq(p.a, w.seq);
+            int lo = 0, n = row_tiles<PAGED>(p, q);
+            int64_t before = 0;
+            while (n > 1) {
+                const int step = (n + 31) / 32, r = lo + lane * step;
+                const int64_t x = lane * step < n ? units_before<PAGED>(p, q, r) : INT64_MAX;
+                const int k = __popc(__ballot_sync(0xffffffffu, x <= at)) - 1;
+                before = __shfl_sync(0xffffffffu, x, k);
+                lo += k * step;
+                n = min(step, n - k * step);
             }
             w.r = lo;
-            w.off = at - units_before<PAGED>(p, q, lo);
+            w.off = at - before;
             return w;
         }
         at -= __shfl_sync(0xffffffffu, upto, 31);
@@ -162,23 +170,31 @@ __device__ __forceinline__ Place find_unit(const Params &p, int64_t at) {
 }
 __device__ __forceinline__ int64_t share_of(const Params &p, int64_t total) { return max((int64_t)p.min_units, (total + p.ctas - 1) / p.ctas); }
 
-// A stretch of the key tiles of one row tile
+// A stretch of the key tiles of one row tile, as the copying warp tells it to the others
 struct Segment {
-    ServeSeq sq;
-    int seq, kvh, r, n, t0, t1;   // key tiles [t0, t1) of n
+    int seq, kvh, token0;         // the row tile's first token within the sequence
+    int q0, k0, nq, nk;           // the sequence
+    int n, t0, t1;                // key tiles [t0, t1) of n; t0 = -1: no more
     int special;                  // tiles from here on are
+    __device__ __forceinline__ int ctx() const { return nk - nq; }   // keys in front of the sequence's first query
 };
-// The stretches of a CTA, the same for all of its warps
+constexpr int SEG_RING = 4;
 template <bool PAGED>
 struct Walk {
     Place at;
     int64_t left;
+    int loaded = -1, tiles = 0;   // the sequence at hand and its row tiles
+    ServeSeq sq;
     __device__ __forceinline__ bool next(const Params &p, Segment &g) {
         while (left > 0 && at.seq < p.a.seqs) {
-            const ServeSeq sq = serve_seq(p.a, at.seq);
-            if (at.r >= row_tiles<PAGED>(p, sq)) {
+            if (loaded != at.seq) {
+                sq = serve_seq(p.a, at.seq);
+                tiles = row_tiles<PAGED>(p, sq);
+                loaded = at.seq;
+            }
+            if (at.r >= tiles) {
                 at.r = 0;
-                if (row_tiles<PAGED>(p, sq) == 0 || ++at.kvh == p.a.kv_heads) {
+                if (tiles == 0 || ++at.kvh == p.a.kv_heads) {
                     at.kvh = 0;
                     at.seq++;
                 }
@@ -186,16 +202,18 @@ struct Walk {
             }
             const int n = key_tiles<PAGED>(p, sq, at.r);
             const int64_t take = min(left, n + OVERHEAD - at.off), off = at.off;
-            g.sq = sq;
             g.seq = at.seq;
             g.kvh = at.kvh;
-            g.r = at.r;
+            g.token0 = at.r * p.tt;
+            g.q0 = (int)sq.q0;
+            g.k0 = (int)sq.k0;
+            g.nq = sq.nq;
+            g.nk = (int)sq.nk;
             g.n = n;
             g.t0 = (int)min(off, (int64_t)n);
             g.t1 = (int)min(off + take, (int64_t)n);
             // keys that every row of the unit sees: the context, or what its first token sees
-            const int64_t all = PAGED ? sq.nk - sq.nq : max((int64_t)0, (int64_t)at.r * p.tt + sq.nk - sq.nq + 1);
-            g.special = (int)(all / T);
+            g.special = (PAGED ? g.ctx() : max(0, g.token0 + g.ctx() + 1)) / T;
             left -= take;
             at.off += take;
             if (at.off == n + OVERHEAD) {
@@ -208,28 +226,61 @@ struct Walk {
     }
 };
 
-// What a row sees: keys up to `lim`, or (PAGED) the context and the drafts of `bits`
+// What a row sees: keys up to `lim` (-1: none), or (PAGED, where lim is not -1) the context and the drafts of `bits`
 struct RowView {
-    int64_t lim;
+    int lim;
     uint64_t bits;
 };
 template <bool PAGED>
-__device__ __forceinline__ bool sees(const RowView &v, int64_t ctx, int64_t key) {
+__device__ __forceinline__ bool sees(const RowView &v, int ctx, int key) {
     if (!PAGED) return key <= v.lim;
     return key < ctx ? v.lim >= 0 : key - ctx < 64 && ((v.bits >> (key - ctx)) & 1);
 }
 // bit i: the row sees key key0 + i
 template <bool PAGED>
-__device__ __forceinline__ uint32_t seen32(const RowView &v, int64_t ctx, int64_t key0) {
+__device__ __forceinline__ uint32_t seen32(const RowView &v, int ctx, int key0) {
     if (!PAGED) {
-        const int64_t n = v.lim - key0 + 1;
-        return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << (int)n) - 1u);
+        const int n = v.lim - key0 + 1;
+        return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
     }
     if (v.lim < 0) return 0u;
-    const int64_t d = key0 - ctx;   // draft of bit 0
+    const int d = key0 - ctx;   // draft of bit 0
     if (d <= -32) return 0xffffffffu;
-    if (d < 0) return ((1u << (int)-d) - 1u) | (uint32_t)(v.bits << (int)-d);
-    return d < 64 ? (uint32_t)(v.bits >> (int)d) : 0u;
+    if (d < 0) return ((1u << -d) - 1u) | (uint32_t)(v.bits << -d);
+    return d < 64 ? (uint32_t)(v.bits >> d) : 0u;
+}
+// Parents of drafts lane and lane + 32 of a sequence, and from them the ancestors of draft i (serve_ancestors of all 64 by doubling:
+// a step joins the ancestors of where the walk stands and doubles its stride)
+__device__ __forceinline__ int2 load_parents(const ServeAttn &a, int seq, int count) {
+    const int32_t *parents = a.parents + (int64_t)seq * a.drafts;
+    const int lane = threadIdx.x & 31;
+    return make_int2(lane < count ? parents[lane] : -1, lane + 32 < count ? parents[lane + 32] : -1);
+}
+__device__ __forceinline__ uint64_t ancestors_of(int2 up, int i, int *err) {
+    const int lane = threadIdx.x & 31;
+    if ((up.x < -1 || up.x >= lane || up.y < -1 || up.y >= lane + 32) && err) report_error(err, TLB_ERR_INDEX);
+    if (up.x < -1 || up.x >= lane) up.x = -1;
+    if (up.y < -1 || up.y >= lane + 32) up.y = -1;
+    uint32_t x0 = 1u << lane, y0 = 0, y1 = 1u << lane;   // masks of drafts lane (only drafts below 32) and lane + 32
+    auto at = [&](uint32_t lo, uint32_t hi, int j) {     // the value of draft j, by its lane
+        const uint32_t a = __shfl_sync(0xffffffffu, lo, j & 31), b = __shfl_sync(0xffffffffu, hi, j & 31);
+        return j < 32 ? a : b;
+    };
+#pragma unroll
+    for (int step = 0; step < 6; step++) {
+        const uint32_t a0 = at(x0, y0, up.x), b0 = at(x0, y0, up.y), b1 = at(0u, y1, up.y);
+        const int ux = (int)at((uint32_t)up.x, (uint32_t)up.y, up.x), uy = (int)at((uint32_t)up.x, (uint32_t)up.y, up.y);
+        if (up.x >= 0) {
+            x0 |= a0;
+            up.x = ux;
+        }
+        if (up.y >= 0) {
+            y0 |= b0;
+            y1 |= b1;
+            up.y = uy;
+        }
+    }
+    return (uint64_t)at(x0, y0, i) | (uint64_t)at(0u, y1, i) << 32;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -256,11 +307,12 @@ __device__ __forceinline__ uint32_t round2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// a += the low half of w, b += the high one, in f32
-template <bool BF16>
-__device__ __forceinline__ void add_halves(uint32_t w, float &a, float &b) {
-    if (BF16) asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.bf16 %0, l, %0;\n\tadd.rn.f32.bf16 %1, h, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(w));
-    else asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.f16 %0, l, %0;\n\tadd.rn.f32.f16 %1, h, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(w));
+__device__ __forceinline__ void add2(uint64_t &s, float a, float b) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(pack2(a, b))); }
+__device__ __forceinline__ float total2(uint64_t s, uint64_t t) {
+    float a, b;
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(t));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(s));
+    return a + b;
 }
 __device__ __forceinline__ void ld32(uint32_t taddr, float *x) {
     uint32_t *r = reinterpret_cast<uint32_t *>(x);
@@ -290,9 +342,29 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(HALF_BYTES >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-// ---- rows of special tiles whose values are not all finite: key by key in f32 (one thread per row)
+// A row's pieces of 16 bytes (32 columns: four of them) turned around among four lanes: piece i is then row (lane & ~3) + i's, its part lane & 3,
+// so that four lanes write 64 bytes of a row side by side instead of 32 lanes to 32 rows
+__device__ __forceinline__ void turn4(uint4 (&w)[4]) {
+    const int lane = threadIdx.x & 31;
+    auto swap = [&](uint4 &a, uint4 &b, int mask) {   // the lane with the bit gives a and takes into it, the other one b
+        const bool up = lane & mask;
+        uint4 x = up ? a : b;
+        x.x = __shfl_xor_sync(0xffffffffu, x.x, mask);
+        x.y = __shfl_xor_sync(0xffffffffu, x.y, mask);
+        x.z = __shfl_xor_sync(0xffffffffu, x.z, mask);
+        x.w = __shfl_xor_sync(0xffffffffu, x.w, mask);
+        if (up) a = x;
+        else b = x;
+    };
+    swap(w[0], w[1], 1);
+    swap(w[2], w[3], 1);
+    swap(w[0], w[2], 2);
+    swap(w[1], w[3], 2);
+}
+
+// ---- a row whose segment has a special tile with values that are not finite: key by key in f32, one thread per row
 template <typename E, bool PAGED>
-__device__ __noinline__ float slow_score(const ServeAttn &a, const ServeSeq &sq, int seq, int kvh, const char *q, int64_t key) {
+__device__ __noinline__ float slow_score(const ServeAttn &a, const ServeSeq &sq, int seq, int kvh, const char *q, int key) {
     const ServeRow at = serve_kv_row<PAGED>(a, seq, sq, kvh, key);
     float s = 0.f;
     if (!at.k) return -CUDART_INF_F;
@@ -305,33 +377,52 @@ __device__ __noinline__ float slow_score(const ServeAttn &a, const ServeSeq &sq,
     }
     return s;
 }
-template <typename E, bool PAGED>
-__device__ __noinline__ void slow_stats(const Params &p, const Segment &g, const RowView &v, const char *q, float &m, float &l) {
-    const int64_t ctx = g.sq.nk - g.sq.nq, k1 = min(g.sq.nk, (int64_t)g.t1 * T);
-    m = -CUDART_INF_F;
-    l = 0.f;
-    for (int64_t key = (int64_t)g.t0 * T; key < k1; key++)
-        if (sees<PAGED>(v, ctx, key)) m = fmaxf(m, slow_score<E, PAGED>(p.a, g.sq, g.seq, g.kvh, q, key) * p.scale_log2);
-    const float ref = m == -CUDART_INF_F ? 0.f : m;
-    for (int64_t key = (int64_t)g.t0 * T; key < k1; key++)
-        if (sees<PAGED>(v, ctx, key)) l += ex2(slow_score<E, PAGED>(p.a, g.sq, g.seq, g.kvh, q, key) * p.scale_log2 - ref);
-    m = ref;
-}
-// columns [c0, c0 + 32) of the unnormalised result
-template <typename E, bool PAGED>
-__device__ __noinline__ void slow_columns(const Params &p, const Segment &g, const RowView &v, const char *q, float m, int c0, float *o) {
-    const int64_t ctx = g.sq.nk - g.sq.nq, k1 = min(g.sq.nk, (int64_t)g.t1 * T);
-    for (int i = 0; i < 32; i++) o[i] = 0.f;
-    for (int64_t key = (int64_t)g.t0 * T; key < k1; key++) {
-        if (!sees<PAGED>(v, ctx, key)) continue;
-        const ServeRow at = serve_kv_row<PAGED>(p.a, g.seq, g.sq, g.kvh, key);
-        if (!at.v) continue;
-        const float w = ex2(slow_score<E, PAGED>(p.a, g.sq, g.seq, g.kvh, q, key) * p.scale_log2 - m);
-        for (int c = 0; c < 4; c++) {
-            if (c0 + c * 8 >= p.a.hs) break;
+// part: null where the segment is a whole row tile, else where its (m, l) and sums go (rows of them)
+template <typename E, bool PAGED, int HSP>
+__device__ __noinline__ void slow_row(const Params &p, const Segment &g, RowView v, int token, int head, float *part, int rows, int prow) {
+    ServeSeq sq;
+    sq.q0 = g.q0;
+    sq.k0 = g.k0;
+    sq.nq = g.nq;
+    sq.nk = g.nk;
+    sq.ok = true;
+    const char *q = (const char *)p.a.q + (int64_t)(g.q0 + token) * p.a.q_stride + (int64_t)head * p.a.hs * 2;
+    char *dst = (char *)p.a.out + (int64_t)(g.q0 + token) * p.a.out_stride + (int64_t)head * p.a.hs * 2;
+    const int ctx = g.ctx(), k0 = g.t0 * T, k1 = min((int64_t)g.nk, (int64_t)g.t1 * T);
+    float m = -CUDART_INF_F, l = 0.f;
+    for (int key = k0; key < k1; key++)
+        if (sees<PAGED>(v, ctx, key)) m = fmaxf(m, slow_score<E, PAGED>(p.a, sq, g.seq, g.kvh, q, key) * p.scale_log2);
+    if (m == -CUDART_INF_F) m = 0.f;
+    for (int key = k0; key < k1; key++)
+        if (sees<PAGED>(v, ctx, key)) l += ex2(slow_score<E, PAGED>(p.a, sq, g.seq, g.kvh, q, key) * p.scale_log2 - m);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (part) {
+        part[prow * 2] = m;
+        part[prow * 2 + 1] = l;
+    }
+    for (int c0 = 0; c0 < p.a.hs; c0 += 8) {
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = 0.f;
+        for (int key = k0; key < k1; key++) {
+            if (!sees<PAGED>(v, ctx, key)) continue;
+            const ServeRow at = serve_kv_row<PAGED>(p.a, g.seq, sq, g.kvh, key);
+            if (!at.v) continue;
+            const float w = ex2(slow_score<E, PAGED>(p.a, sq, g.seq, g.kvh, q, key) * p.scale_log2 - m);
             float y[8];
-            serve_unpack<E>(*reinterpret_cast<const uint4 *>(at.v + (c0 + c * 8) * 2), y);
-            for (int e = 0; e < 8; e++) o[c * 8 + e] = fmaf(w, y[e], o[c * 8 + e]);
+            serve_unpack<E>(*reinterpret_cast<const uint4 *>(at.v + c0 * 2), y);
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = fmaf(w, y[e], o[e]);
+        }
+        if (part) {
+            float4 *at = reinterpret_cast<float4 *>(part + rows * 2) + (size_t)(c0 / 4) * rows + prow;
+            at[0] = make_float4(o[0], o[1], o[2], o[3]);
+            at[rows] = make_float4(o[4], o[5], o[6], o[7]);
+        } else {
+            E r[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) r[e] = serve_round<E>(o[e] * inv);
+            *reinterpret_cast<uint4 *>(dst + c0 * 2) = *reinterpret_cast<const uint4 *>(r);
         }
     }
 }
@@ -351,7 +442,8 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     __shared__ uint32_t tmem_base_s;
     __shared__ int s_fail;
     __shared__ volatile int slow_ring[SLOW_RING];   // segment + 1 of those whose special tiles hold values that are not finite
-    __shared__ Walk<PAGED> walks[sat::THREADS / 32];   // in shared memory between segments: the streams' registers are full of scores
+    __shared__ Segment segs[SEG_RING];
+    __shared__ uint64_t bar_seg[SEG_RING], bar_segfree[SEG_RING];
     __shared__ float pair_ml[2][T][2];
     volatile int *fail = &s_fail;
 
@@ -373,21 +465,16 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             mbar_init(&bar_o[i], 1);
         }
         mbar_init(&bar_od, 8);
+        for (int i = 0; i < SEG_RING; i++) {
+            mbar_init(&bar_seg[i], 1);
+            mbar_init(&bar_segfree[i], 11);   // every warp but the one that writes
+        }
         s_fail = 0;
         for (int i = 0; i < SLOW_RING; i++) slow_ring[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) tmem_alloc(&tmem_base_s, 512);
     griddep_wait();
-    if (warp == 3) {
-        const int64_t total = total_units<PAGED>(p), share = share_of(p, total), a0 = share * blockIdx.x;
-        const int64_t mine = min(share, total - a0);
-        const Place w = mine > 0 ? find_unit<PAGED>(p, a0) : Place{p.a.seqs, 0, 0, 0};
-        if (lane < sat::THREADS / 32) {
-            walks[lane].at = w;
-            walks[lane].left = mine;
-        }
-    }
     if (warp == 2 && blockIdx.x == 0 && p.a.err) {
         for (int s = lane; s < p.a.seqs; s += 32)
             if (!serve_seq(p.a, s).ok) report_error(p.a.err, TLB_ERR_INDEX);
@@ -397,19 +484,39 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     tc_fence_after();
     const uint32_t tmem = tmem_base_s;
     Segment g;
+    int g_at = 0;   // segments seen
     auto next = [&]() {
-        Walk<PAGED> w = walks[warp];
+        const int r = g_at % SEG_RING;
+        mbar_wait_nap(&bar_seg[r], (uint32_t)(g_at / SEG_RING) & 1u, fail, 0);
+        g = segs[r];
         __syncwarp();
-        const bool more = w.next(p, g);
-        if (lane == 0) walks[warp] = w;
-        __syncwarp();
-        return more;
+        if (lane == 0) mbar_arrive(&bar_segfree[r]);
+        g_at++;
+        return g.t0 >= 0 && !*fail;
     };
 
     if (warp == 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
         // ---- copies. The keys of a segment's first tiles are on their way before its queries, whose room the segment in front still uses.
+        Walk<PAGED> walk;
+        {
+            int64_t seq0;
+            const int64_t total = total_units<PAGED>(p, seq0), share = share_of(p, total), first = share * blockIdx.x;
+            walk.left = min(share, total - first);
+            if (walk.left > 0) walk.at = find_unit<PAGED>(p, first, seq0);
+        }
+        auto tell = [&]() {
+            const int r = g_at % SEG_RING;
+            mbar_wait_nap(&bar_segfree[r], (uint32_t)(g_at / SEG_RING + 1) & 1u, fail, 32);
+            if (lane == 0) {
+                segs[r] = g;
+                mbar_arrive(&bar_seg[r]);
+            }
+            g_at++;
+        };
         int tile = 0, seg = 0;
-        while (next()) {
+        while (walk.next(p, g)) {
+            tell();
             if (g.t1 == g.t0) continue;   // a row tile that sees nothing has no part in the pipeline's counts
             bool have_q = false;
             auto load_q = [&]() {
@@ -418,7 +525,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                     mbar_expect_tx(&bar_q, (uint32_t)(NQ * HALVES * 128 * p.group * p.tpt));
                     for (int x = 0; x < NQ; x++)
                         for (int h = 0; h < HALVES; h++)
-                            tma_3d(qs + x * TILE + h * HALF_BYTES, &p.q, h * 64, g.kvh * p.group, (int)(g.sq.q0 + (int64_t)g.r * p.tt + x * p.tpt), &bar_q);
+                            tma_3d(qs + x * TILE + h * HALF_BYTES, &p.q, h * 64, g.kvh * p.group, g.q0 + g.token0 + x * p.tpt, &bar_q);
                 }
                 have_q = true;
             };
@@ -428,7 +535,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 const uint32_t free_parity = (uint32_t)(tile / NS + 1) & 1u;
                 if (!PAGED) {
                     if (lane == 0) {
-                        const int z = (int)(g.sq.k0 + (int64_t)j * T);
+                        const int z = g.k0 + j * T;
                         mbar_wait_nap(&bar_kfree[s], free_parity, fail, 32);
                         mbar_expect_tx(&bar_k[s], TILE);
                         for (int h = 0; h < HALVES; h++) tma_3d(ks + s * TILE + h * HALF_BYTES, &p.k, h * 64, g.kvh, z, &bar_k[s]);
@@ -441,10 +548,10 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                     const int rows = min(p.a.block_size, T), boxes = T / rows;   // 1 to 16 pages
                     int row = p.pool_rows;
                     if (lane < boxes) {
-                        const int64_t key = (int64_t)j * T + lane * rows;
-                        if (key < g.sq.nk) {
+                        const int key = j * T + lane * rows;
+                        if (key < g.nk) {
                             const int32_t blk = p.a.tables[(int64_t)g.seq * p.a.max_blocks + key / p.a.block_size];
-                            if (blk >= 0 && blk < p.a.pool_blocks) row = (blk * p.a.kv_heads + g.kvh) * p.a.block_size + (int)(key % p.a.block_size);
+                            if (blk >= 0 && blk < p.a.pool_blocks) row = (blk * p.a.kv_heads + g.kvh) * p.a.block_size + key % p.a.block_size;
                             else if (p.a.err) report_error(p.a.err, TLB_ERR_INDEX);
                         }
                     }
@@ -466,6 +573,8 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             __syncwarp();
             seg++;
         }
+        g.t0 = -1;
+        tell();
         // only after a wait has given up: this CTA's copies are over before its shared memory is
         if (*fail && lane == 0) {
             mbar_wait_limit(&bar_q, 0, 1u << 12);
@@ -477,6 +586,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             }
         }
     } else if (warp == 1) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
         // ---- MMA issue: step i is stream i & 1; S of step i + 2 follows O of step i, which has read the P that it overwrites
         const bool leader = elect_one();
         int tile = 0, seg = 0;
@@ -525,6 +635,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             seg++;
         }
     } else if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
         // ---- every tile of values passes here, in order, on its way to the MMAs. Special ones: rows behind the end become zero, the others are
         // looked through
         int tile = 0, seg = 0;
@@ -534,7 +645,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 const int s = tile % NS;
                 mbar_wait_nap(&bar_v[s], (uint32_t)(tile / NS) & 1u, fail, 0);
                 if (j >= g.special) {
-                    const int live = (int)min((int64_t)T, g.sq.nk - (int64_t)j * T);
+                    const int live = min(T, g.nk - j * T);
                     uint4 *v = reinterpret_cast<uint4 *>(vs + s * TILE);
                     constexpr uint32_t EXP = BF16 ? 0x7f807f80u : 0x7c007c00u;
                     uint32_t odd = 0;
@@ -556,6 +667,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             seg++;
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_STREAMS));
         // ---- the streams
         const int x = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
@@ -563,13 +675,15 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         int seg = 0;
         uint32_t done[2] = {0, 0};   // tiles of either stream so far
         while (next()) {
-            const int64_t ctx = g.sq.nk - g.sq.nq;
-            const int token = g.r * p.tt + (SHARE ? x * p.tpt : 0) + row / p.group, head = g.kvh * p.group + row % p.group;
-            const bool live_row = row < p.tpt * p.group && token < (PAGED ? p.a.drafts : g.sq.nq);
+            const int ctx = g.ctx();
+            const int token = g.token0 + (SHARE ? x * p.tpt : 0) + row / p.group, head = g.kvh * p.group + row % p.group;
+            const bool live_row = row < p.tpt * p.group && token < (PAGED ? p.a.drafts : g.nq);
             RowView view;
             view.bits = 0;
-            view.lim = live_row && token < g.sq.nq ? ctx + token : -1;
-            if (PAGED && view.lim >= 0) view.bits = serve_ancestors(p.a, g.seq, token);
+            view.lim = live_row && token < g.nq ? ctx + token : -1;
+            int2 parents;
+            if (PAGED) parents = load_parents(p.a, g.seq, g.nq);   // on their way while the tiles of the context are looked at
+            bool have_bits = false;
             const int n = g.t1 - g.t0;
             const int mine = SHARE ? n : (n + 1 - x) / 2, other = SHARE ? n : (n + x) / 2;
             float m_ref = 0.f, l = 0.f;
@@ -583,18 +697,24 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 for (int c = 0; c < 4; c++) ld32(s_at + 32 * c, y + 32 * c);
                 tmem_ld_wait();
                 if (j >= g.special) {
+                    if (PAGED && !have_bits) {
+                        view.bits = ancestors_of(parents, token & 63, p.a.err);
+                        have_bits = true;
+                    }
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
-                        const uint32_t seen = seen32<PAGED>(view, ctx, (int64_t)j * T + 32 * c);
+                        const uint32_t seen = seen32<PAGED>(view, ctx, j * T + 32 * c);
 #pragma unroll
                         for (int e = 0; e < 32; e++)
                             if (!((seen >> e) & 1u)) y[32 * c + e] = -CUDART_INF_F;
                     }
                 }
-                float mx = y[0];
+                float mxs[4] = {y[0], y[1], y[2], y[3]};   // four chains
 #pragma unroll
-                for (int e = 1; e < T; e++) mx = fmaxf(mx, y[e]);
-                mx *= p.scale_log2;
+                for (int e = 4; e < T; e += 4)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) mxs[c] = fmaxf(mxs[c], y[e + c]);
+                const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * p.scale_log2;
                 float alpha = 1.f;
                 if (!have_ref) {
                     if (mx != -CUDART_INF_F) {
@@ -620,7 +740,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                     l *= alpha;
                 }
                 const uint64_t sc = pack2(p.scale_log2, p.scale_log2), ref = pack2(-m_ref, -m_ref);
-                float sum0 = 0.f, sum1 = 0.f;
+                uint64_t sums[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     uint32_t w[32];
@@ -628,12 +748,14 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                     for (int e = 0; e < 32; e++) {
                         float a = y[64 * c + 2 * e], b = y[64 * c + 2 * e + 1];
                         fma2(a, b, sc, ref);
-                        w[e] = round2<BF16>(ex2(a), ex2(b));
-                        add_halves<BF16>(w[e], sum0, sum1);
+                        a = ex2(a);
+                        b = ex2(b);
+                        add2(sums[e & 1], a, b);
+                        w[e] = round2<BF16>(a, b);
                     }
                     st32(s_at + 32 * c, w);
                 }
-                l += sum0 + sum1;
+                l += total2(sums[0], sums[1]);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -646,79 +768,79 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             if (!SHARE && other > 0) mbar_wait_nap(&bar_o[x ^ 1], (done[x ^ 1] - 1) & 1u, fail, 0);
             tc_fence_after();
             const bool slow = n > 0 && slow_ring[seg % SLOW_RING] == seg + 1;
-            const char *q = (const char *)p.a.q + (g.sq.q0 + token) * p.a.q_stride + (int64_t)head * p.a.hs * 2;
-            float f_mine = 1.f, f_other = 0.f;
-            if (slow) {
-                if (view.lim >= 0) slow_stats<E, PAGED>(p, g, view, q, m_ref, l);
-                __syncwarp();
-            } else if (!SHARE) {
-                pair_ml[x][row][0] = have_ref ? m_ref : -CUDART_INF_F;
-                pair_ml[x][row][1] = l;
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                const float m2 = pair_ml[x ^ 1][row][0], l2 = pair_ml[x ^ 1][row][1], m1 = have_ref ? m_ref : -CUDART_INF_F;
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                m_ref = fmaxf(m1, m2);
-                if (m_ref == -CUDART_INF_F) m_ref = 0.f;
-                f_mine = ex2(m1 - m_ref);
-                f_other = ex2(m2 - m_ref);
-                l = l * f_mine + l2 * f_other;
-            }
-            if (view.lim < 0) l = 0.f;   // a row that sees nothing, or no token's
             const bool whole = g.t0 == 0 && g.t1 == g.n;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
             float *part = whole ? nullptr : p.partial + ((size_t)blockIdx.x * 2 + (g.t0 > 0 ? 0 : 1)) * (NQ * T) * (2 + HSP);
             const int prow = (SHARE ? x * T : 0) + row;
-            if (!whole && (SHARE || x == 0)) {
-                part[prow * 2] = m_ref;
-                part[prow * 2 + 1] = l;
-            }
-            // SHARE: a thread writes its row; else the streams take half of the columns each
-            constexpr int COLS = SHARE ? HSP : HSP / 2;
-            const int c_first = SHARE ? 0 : x * COLS;
-#pragma unroll 1
-            for (int c0 = c_first; c0 < c_first + COLS; c0 += 32) {
-                float o[32];
+            if (slow) {
+                if (PAGED && !have_bits) view.bits = ancestors_of(parents, token & 63, p.a.err);
+                if (live_row && (SHARE || x == 0)) slow_row<E, PAGED, HSP>(p, g, view, token, head, part, NQ * T, prow);
                 __syncwarp();
-                if (slow) {
-                    if (view.lim >= 0) slow_columns<E, PAGED>(p, g, view, q, m_ref, c0, o);
-                    __syncwarp();
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = 0.f;
-                    if (mine > 0) {
-                        ld32(o_at + c0, o);
-                        tmem_ld_wait();
-                    }
-                    if (!SHARE) {
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] *= f_mine;
-                        if (other > 0) {
-                            float o2[32];
-                            ld32(lanes + O_COL + (uint32_t)((x ^ 1) * T) + c0, o2);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] = fmaf(o2[e], f_other, o[e]);
-                        }
-                    }
+            } else {
+                float f_mine = 1.f, f_other = 0.f;
+                if (!SHARE) {
+                    pair_ml[x][row][0] = have_ref ? m_ref : -CUDART_INF_F;
+                    pair_ml[x][row][1] = l;
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    const float m2 = pair_ml[x ^ 1][row][0], l2 = pair_ml[x ^ 1][row][1], m1 = have_ref ? m_ref : -CUDART_INF_F;
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    m_ref = fmaxf(m1, m2);
+                    if (m_ref == -CUDART_INF_F) m_ref = 0.f;
+                    f_mine = ex2(m1 - m_ref);
+                    f_other = ex2(m2 - m_ref);
+                    l = l * f_mine + l2 * f_other;
                 }
-                if (view.lim < 0) {
-#pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = 0.f;
-                }
+                if (view.lim < 0) l = 0.f;   // a row that sees nothing, or no token's
+                const float inv = l == 0.f ? 0.f : 1.f / l;
                 if (whole) {
-                    if (live_row) {
-                        char *dst = (char *)p.a.out + (g.sq.q0 + token) * p.a.out_stride + (int64_t)head * p.a.hs * 2;
+                    f_mine *= inv;
+                    f_other *= inv;
+                } else if (SHARE || x == 0) {
+                    *reinterpret_cast<float2 *>(part + prow * 2) = make_float2(m_ref, l);
+                }
+                // where the rows of this lane's four go (turn4)
+                const int64_t at = (int64_t)(g.q0 + token) * p.a.out_stride + (int64_t)head * p.a.hs * 2;
+                char *dst[4];
+                bool ok[4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (c0 + 8 * e < p.a.hs)
-                                *reinterpret_cast<uint4 *>(dst + (c0 + 8 * e) * 2) =
-                                    make_uint4(round2<BF16>(o[8 * e] * inv, o[8 * e + 1] * inv), round2<BF16>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                               round2<BF16>(o[8 * e + 4] * inv, o[8 * e + 5] * inv), round2<BF16>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+                for (int i = 0; i < 4; i++) {
+                    dst[i] = (char *)p.a.out + __shfl_sync(0xffffffffu, at, (lane & ~3) + i) + (lane & 3) * 16;
+                    ok[i] = __shfl_sync(0xffffffffu, (int)live_row, (lane & ~3) + i);
+                }
+                // SHARE: a stream writes its rows; else half of the columns each
+                constexpr int COLS = SHARE ? HSP : HSP / 2;
+                const int c_first = SHARE ? 0 : x * COLS;
+#pragma unroll 1
+                for (int c0 = c_first; c0 < c_first + COLS; c0 += 32) {
+                    __syncwarp();
+                    float o[32];
+                    ld32(o_at + c0, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = mine > 0 && view.lim >= 0 ? o[e] * f_mine : 0.f;
+                    if (!SHARE) {
+                        float o2[32];
+                        ld32(lanes + O_COL + (uint32_t)((x ^ 1) * T) + c0, o2);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = other > 0 && view.lim >= 0 ? fmaf(o2[e], f_other, o[e]) : o[e];
                     }
-                } else if (live_row) {
-                    float4 *dst = reinterpret_cast<float4 *>(part + NQ * T * 2 + (size_t)prow * HSP + c0);
+                    if (whole) {
+                        uint4 w[4];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        for (int i = 0; i < 4; i++)
+                            w[i] = make_uint4(round2<BF16>(o[8 * i], o[8 * i + 1]), round2<BF16>(o[8 * i + 2], o[8 * i + 3]), round2<BF16>(o[8 * i + 4], o[8 * i + 5]),
+                                              round2<BF16>(o[8 * i + 6], o[8 * i + 7]));
+                        turn4(w);
+                        if (c0 + (lane & 3) * 8 < p.a.hs) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (ok[i]) *reinterpret_cast<uint4 *>(dst[i] + c0 * 2) = w[i];
+                        }
+                    } else if (live_row) {
+                        float4 *to = reinterpret_cast<float4 *>(part + NQ * T * 2) + (size_t)(c0 / 4) * (NQ * T) + prow;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) to[e * NQ * T] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    }
                 }
             }
             tc_fence_before();
@@ -745,8 +867,9 @@ __global__ void __launch_bounds__(128) k_serve_join(const __grid_constant__ sat:
     __shared__ int64_t share_s;
     const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
-        const int64_t total = total_units<PAGED>(p), share = share_of(p, total), end = share * (c + 1);
-        const Place w = end < total ? find_unit<PAGED>(p, end) : Place{p.a.seqs, 0, 0, 0};
+        int64_t seq0;
+        const int64_t total = total_units<PAGED>(p, seq0), share = share_of(p, total), end = share * (c + 1);
+        const Place w = end < total ? find_unit<PAGED>(p, end, seq0) : Place{p.a.seqs, 0, 0, 0};
         if (lane == 0) {
             at_s = w;
             share_s = share;
@@ -759,39 +882,49 @@ __global__ void __launch_bounds__(128) k_serve_join(const __grid_constant__ sat:
     const int n = key_tiles<PAGED>(p, sq, w.r);
     if (w.off >= n) return;   // all of its key tiles lie in this stretch
     const int parts = 1 + (int)((n - w.off + share_s - 1) / share_s);
-    for (int row = blockIdx.y * 8 + warp; row < (int)blockIdx.y * 8 + 8; row += 4) {
-        const int x = row / T, rr = row % T;
-        const int token = w.r * p.tt + x * p.tpt + rr / p.group, head = w.kvh * p.group + rr % p.group;
-        if (rr >= p.tpt * p.group || token >= (PAGED ? p.a.drafts : sq.nq)) continue;
-        float m = -CUDART_INF_F;
-        auto slot = [&](int i) { return p.partial + ((size_t)(c + i) * 2 + (i ? 0 : 1)) * SLOT; };
-        for (int i = lane; i < parts; i += 32) m = fmaxf(m, slot(i)[row * 2 + 1] == 0.f ? -CUDART_INF_F : slot(i)[row * 2]);
+    // 32 rows: a lane's row is its own, a warp's columns a quarter of them
+    const int row = blockIdx.y * 32 + lane, x = row / T, rr = row % T;
+    const int token = w.r * p.tt + x * p.tpt + rr / p.group, head = w.kvh * p.group + rr % p.group;
+    if (rr >= p.tpt * p.group || token >= (PAGED ? p.a.drafts : sq.nq)) return;
+    auto slot = [&](int i) { return p.partial + ((size_t)(c + i) * 2 + (i ? 0 : 1)) * SLOT; };
+    float m = -CUDART_INF_F;
+    for (int i = 0; i < parts; i++) {
+        const float2 ml = *reinterpret_cast<const float2 *>(slot(i) + row * 2);
+        if (ml.y != 0.f) m = fmaxf(m, ml.x);   // else the row sees nothing in this part
+    }
+    if (m == -CUDART_INF_F) m = 0.f;
+    float l = 0.f;
+    float4 o[HSP / 16];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (m == -CUDART_INF_F) m = 0.f;
-        float l = 0.f, o[HSP / 32];
+    for (int e = 0; e < HSP / 16; e++) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < parts; i++) {
+        const float2 ml = *reinterpret_cast<const float2 *>(slot(i) + row * 2);
+        if (ml.y == 0.f) continue;
+        const float f = ex2(ml.x - m);
+        l = fmaf(ml.y, f, l);
+        const float4 *s = reinterpret_cast<const float4 *>(slot(i) + ROWS * 2) + (size_t)(warp * (HSP / 16)) * ROWS + row;
 #pragma unroll
-        for (int e = 0; e < HSP / 32; e++) o[e] = 0.f;
-        for (int i = 0; i < parts; i++) {
-            const float *s = slot(i), li = s[row * 2 + 1];
-            if (li == 0.f) continue;   // a part in which the row sees nothing
-            const float f = ex2(s[row * 2] - m);
-            l = fmaf(li, f, l);
-#pragma unroll
-            for (int e = 0; e < HSP / 32; e++) o[e] = fmaf(s[ROWS * 2 + row * HSP + lane * (HSP / 32) + e], f, o[e]);
+        for (int e = 0; e < HSP / 16; e++) {
+            const float4 y = s[(size_t)e * ROWS];
+            o[e] = make_float4(fmaf(y.x, f, o[e].x), fmaf(y.y, f, o[e].y), fmaf(y.z, f, o[e].z), fmaf(y.w, f, o[e].w));
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        using E = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-        E *dst = reinterpret_cast<E *>((char *)p.a.out + (sq.q0 + token) * p.a.out_stride) + (int64_t)head * p.a.hs;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    char *dst = (char *)p.a.out + (sq.q0 + token) * p.a.out_stride + (int64_t)head * p.a.hs * 2;
 #pragma unroll
-        for (int e = 0; e < HSP / 32; e++)
-            if (lane * (HSP / 32) + e < p.a.hs) dst[lane * (HSP / 32) + e] = serve_round<E>(o[e] * inv);
+    for (int e = 0; e < HSP / 16; e += 2) {
+        const int col = warp * (HSP / 4) + e * 4;
+        if (col < p.a.hs)
+            *reinterpret_cast<uint4 *>(dst + col * 2) = make_uint4(round2<BF16>(o[e].x * inv, o[e].y * inv), round2<BF16>(o[e].z * inv, o[e].w * inv),
+                                                                   round2<BF16>(o[e + 1].x * inv, o[e + 1].y * inv), round2<BF16>(o[e + 1].z * inv, o[e + 1].w * inv));
     }
 }
 
 // ---------------------------------------------------------------- host side
+// The register shares must not exceed what a CTA is launched with, or the streams would wait for theirs for good (serve_attn_tc_configure).
+static bool g_sat_registers = true;
 bool serve_attn_tc_supported(const ServeAttn &a) {
-    if (!tc_available() || a.hs > 128 || a.heads / a.kv_heads > sat::T) return false;
+    if (!g_sat_registers || !tc_available() || a.hs > 128 || a.heads / a.kv_heads > sat::T) return false;
     if (a.paged) return a.block_size >= 8 && a.pool_blocks > 0 && a.pool_blocks * a.kv_heads * a.block_size < 0x7fffffff;
     return a.kv_rows > 0;
 }
@@ -811,11 +944,14 @@ uint64_t serve_attn_tc_scratch_bytes(const ServeAttn &a, int sm_count) {
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
 static cudaError_t sat_launch(const sat::Params &p, int ctas, cudaStream_t st) {
     cudaError_t e = launch_pdl(k_serve_attn_tc<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas), dim3(sat::THREADS), sat::smem_bytes(HSP, SHARE), st, p);
-    if (e == cudaSuccess && ctas > 1) e = launch_pdl(k_serve_join<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas - 1, (SHARE ? 2 : 1) * sat::T / 8), dim3(128), 0, st, p);
+    if (e == cudaSuccess && ctas > 1) e = launch_pdl(k_serve_join<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas - 1, (SHARE ? 2 : 1) * sat::T / 32), dim3(128), 0, st, p);
     return e;
 }
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
 static void sat_configure() {
+    cudaFuncAttributes at;
+    if (cudaFuncGetAttributes(&at, k_serve_attn_tc<HSP, BF16, PAGED, SHARE>) != cudaSuccess || at.numRegs * sat::THREADS < 128 * sat::REGS_ROLES + 256 * sat::REGS_STREAMS)
+        g_sat_registers = false;
     cudaFuncSetAttribute(k_serve_attn_tc<HSP, BF16, PAGED, SHARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, sat::smem_bytes(HSP, SHARE));
 }
 void serve_attn_tc_configure() {
