@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
+#include <type_traits>
 
 #include "kernels.h"
 #include "pdl.cuh"
@@ -46,42 +47,77 @@ __device__ __forceinline__ float unorder(int o) { return __int_as_float(o ^ ((o 
 struct Sums {
     float m, s, t;
 };
-// d = x - m is at least -1e4 in products with exp(d), which is 0 there: no 0 x inf
-__device__ __forceinline__ Sums join(const Sums &a, const Sums &b) {
-    const float m = fmaxf(a.m, b.m), mu = m == -CUDART_INF_F ? 0.f : m;
-    const float da = fmaxf(a.m - mu, -1e4f), db = fmaxf(b.m - mu, -1e4f);
-    const float fa = ex2(da * LOG2E), fb = ex2(db * LOG2E);
-    return {m, a.s * fa + b.s * fb, fa * (a.t + da * a.s) + fb * (b.t + db * b.s)};
+__device__ __forceinline__ float warp_max(float x) {   // NaNs have no part in it
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
 }
-__device__ __forceinline__ Sums join_block(Sums v, Sums *sh) {
+// d = x - m is at least -1e4 in products with exp(d), which is 0 there: no 0 x inf
+__device__ __forceinline__ void move_to(Sums &v, float m) {   // the sums with another maximum
+    const float d = fmaxf(v.m - (m == -CUDART_INF_F ? 0.f : m), -1e4f), f = ex2(d * LOG2E);
+    v.t = f * fmaf(d, v.s, v.t);
+    v.s *= f;
+    v.m = m;
+}
+__device__ __forceinline__ Sums join_warp(Sums v) {   // in every lane
+    move_to(v, warp_max(v.m));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        Sums w;
-        w.m = __shfl_xor_sync(0xffffffffu, v.m, o);
-        w.s = __shfl_xor_sync(0xffffffffu, v.s, o);
-        w.t = __shfl_xor_sync(0xffffffffu, v.t, o);
-        v = join(v, w);
+        v.s += __shfl_xor_sync(0xffffffffu, v.s, o);
+        v.t += __shfl_xor_sync(0xffffffffu, v.t, o);
     }
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = sh[0];
-#pragma unroll
-    for (int w = 1; w < WARPS; w++) v = join(v, sh[w]);
     return v;
 }
-// A row's 16-byte pieces start `shift` elements in front of it; only whole pieces inside the row are read as such.
+// A row's 16-byte pieces start `shift` elements in front of it; only whole pieces inside the row are read as such. Outside it: -inf.
 template <typename T>
-__device__ __forceinline__ void load_piece(const T *row, int64_t vocab, int64_t first, float (&x)[Vec<T>::N]) {
+__device__ __forceinline__ uint4 load_piece(const T *row, int vocab, int first) {
     constexpr int N = Vec<T>::N;
-    if (first >= 0 && first + N <= vocab) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(row + first));
-        const T *e = reinterpret_cast<const T *>(&raw);
+    if (first >= 0 && first + N <= vocab) return __ldg(reinterpret_cast<const uint4 *>(row + first));
+    uint32_t w[4];
+    if (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < N; i++) x[i] = value(e[i]);
+        for (int i = 0; i < 4; i++) w[i] = first + i >= 0 && first + i < vocab ? reinterpret_cast<const uint32_t *>(row)[first + i] : 0xff800000u;
     } else {
+        const uint32_t none = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
 #pragma unroll
-        for (int i = 0; i < N; i++) x[i] = first + i >= 0 && first + i < vocab ? value(row[first + i]) : -CUDART_INF_F;
+        for (int i = 0; i < 4; i++) {
+            const int j = first + 2 * i;
+            const uint32_t lo = j >= 0 && j < vocab ? reinterpret_cast<const uint16_t *>(row)[j] : none;
+            const uint32_t hi = j + 1 >= 0 && j + 1 < vocab ? reinterpret_cast<const uint16_t *>(row)[j + 1] : none;
+            w[i] = lo | hi << 16;
+        }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays one
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 template <typename T>
 __device__ __forceinline__ int shift_of(const T *row) { return (int)(((uintptr_t)row & 15) / sizeof(T)); }
@@ -89,8 +125,8 @@ __device__ __forceinline__ int shift_of(const T *row) { return (int)(((uintptr_t
 struct Scan {
     Logprobs a;
     Sums *part;        // [rows][splits]
-    float *seg_max;    // [rows][segs], null: no alternatives asked for
-    int splits, segs, segs_per_split;
+    float *seg_max;    // [rows][turns][UNROLL], null: no alternatives asked for
+    int splits, turns, turns_per_split;
 };
 }  // namespace lp
 
@@ -105,102 +141,164 @@ __global__ void __launch_bounds__(lp::THREADS) k_logprobs_scan(const __grid_cons
     const int64_t row_i = blockIdx.y + (int64_t)blockIdx.z * 65535;
     if (row_i >= p.a.rows) return;
     const T *row = reinterpret_cast<const T *>((const char *)p.a.logits + row_i * p.a.stride);
-    const int shift = shift_of(row);
-    const int s0 = (int)blockIdx.x * p.segs_per_split, s1 = min(p.segs, s0 + p.segs_per_split);
-    Sums v = {-CUDART_INF_F, 0.f, 0.f};
-    for (int seg = s0 + warp; seg < s1; seg += WARPS * UNROLL) {
+    const int shift = shift_of(row), vocab = (int)p.a.vocab;
+    const int q0 = (int)blockIdx.x * p.turns_per_split, q1 = min(p.turns, q0 + p.turns_per_split);
+    // a turn: UNROLL segments in a row; the next one's pieces are on their way while these are added up
+    uint4 raw[UNROLL];
+    auto fetch = [&](int q) {
+        const int first = q * UNROLL * SEG - shift;
+        if (first >= 0 && first + UNROLL * SEG <= vocab) {
+            const uint4 *at = reinterpret_cast<const uint4 *>(row + first) + lane;
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) raw[u] = __ldg(at + 32 * u);
+        } else {
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) raw[u] = load_piece<T>(row, vocab, first + u * SEG + lane * N);
+        }
+    };
+    float m = -CUDART_INF_F;
+    uint64_t sums = 0, prods = 0;   // pairs: s and t of even and odd elements
+    if (q0 + warp < q1) fetch(q0 + warp);
+    for (int q = q0 + warp; q < q1; q += WARPS) {
         float x[UNROLL][N];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
-            const int g = seg + u * WARPS;
-            if (g < s1) {
-                load_piece<T>(row, p.a.vocab, (int64_t)g * SEG + lane * N - shift, x[u]);
-            } else {
+            const T *e = reinterpret_cast<const T *>(&raw[u]);
 #pragma unroll
-                for (int i = 0; i < N; i++) x[u][i] = -CUDART_INF_F;
-            }
+            for (int i = 0; i < N; i++) x[u][i] = value(e[i]);
         }
-        float mx = -CUDART_INF_F;
+        if (q + WARPS < q1) fetch(q + WARPS);
+        float mx = m, mu[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
-            float mu = x[u][0];
+            mu[u] = x[u][0];
 #pragma unroll
-            for (int i = 1; i < N; i++) mu = fmaxf(mu, x[u][i]);
-            if (p.seg_max) {
-                const int best = __reduce_max_sync(0xffffffffu, order(mu));
-                const int g = seg + u * WARPS;
-                if (lane == 0 && g < s1) p.seg_max[row_i * p.segs + g] = unorder(best);
-            }
-            mx = fmaxf(mx, mu);
+            for (int i = 1; i < N; i++) mu[u] = fmaxf(mu[u], x[u][i]);
+            mx = fmaxf(mx, mu[u]);
         }
-        if (mx > v.m) {
-            const float d = fmaxf(v.m - mx, -1e4f), f = ex2(d * LOG2E);
-            v.t = f * (v.t + d * v.s);
-            v.s *= f;
-            v.m = mx;
+        if (p.seg_max) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) mu[u] = warp_max(mu[u]);
+            if (lane == 0) *reinterpret_cast<float4 *>(p.seg_max + (row_i * p.turns + q) * UNROLL) = make_float4(mu[0], mu[1], mu[2], mu[3]);
         }
-        const float m = v.m == -CUDART_INF_F ? 0.f : v.m;
+        if (mx > m) {
+            const float d = fmaxf(m - mx, -1e4f), f = ex2(d * LOG2E);
+            prods = mul2(pack2(f, f), fma2(pack2(d, d), sums, prods));   // as move_to
+            sums = mul2(pack2(f, f), sums);
+            m = mx;
+        }
+        const float ref = m == -CUDART_INF_F ? 0.f : m;
 #pragma unroll
         for (int u = 0; u < UNROLL; u++)
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float d = x[u][i] - m, e = ex2(d * LOG2E);
-                v.s += e;
-                v.t = fmaf(e, fmaxf(d, -1e4f), v.t);
+            for (int i = 0; i < N; i += 2) {
+                const float2 d = unpack2(add2(pack2(x[u][i], x[u][i + 1]), pack2(-ref, -ref)));
+                const uint64_t at = pack2(max_nan(d.x, -1e4f), max_nan(d.y, -1e4f));
+                const float2 a = unpack2(mul2(at, pack2(LOG2E, LOG2E)));
+                const uint64_t e = pack2(ex2(a.x), ex2(a.y));
+                sums = add2(sums, e);
+                prods = fma2(e, at, prods);
             }
     }
-    v = join_block(v, sh);
-    if (threadIdx.x == 0) p.part[row_i * p.splits + blockIdx.x] = v;
+    const float2 s2 = unpack2(sums), t2 = unpack2(prods);
+    Sums v = {m, s2.x + s2.y, t2.x + t2.y};
+    v = join_warp(v);
+    if (lane == 0) sh[warp] = v;
+    __syncthreads();
+    if (warp > 0) return;
+    v = join_warp(lane < WARPS ? sh[lane] : Sums{-CUDART_INF_F, 0.f, 0.f});
+    if (lane == 0) p.part[row_i * p.splits + blockIdx.x] = v;
 }
 
 namespace lp {
-struct Best {
-    int o;         // order() of the value
-    uint32_t id;   // 0xffffffff: none
-};
-constexpr int NONE = INT32_MIN;
-__device__ __forceinline__ bool after(int o, uint32_t id, const Best &last) { return o < last.o || (o == last.o && id > last.id); }
+// A candidate as one number: the larger value first, of equal ones the lower id; 0: none. -inf is no candidate.
+using Key = uint64_t;
+__device__ __forceinline__ Key key_of(float x, uint32_t id) { return x > -CUDART_INF_F ? (uint64_t)((uint32_t)order(x) ^ 0x80000000u) << 32 | (0xffffffffu - id) : 0; }
+__device__ __forceinline__ uint32_t id_of(Key k) { return 0xffffffffu - (uint32_t)k; }
+__device__ __forceinline__ float value_of(Key k) { return unorder((int)((uint32_t)(k >> 32) ^ 0x80000000u)); }
 
-// The k largest of n candidates at(i) -> Best, equal values by rising id, to out[0..k) (id 0xffffffff where they run out). Every thread keeps
-// the best of its share; the winner's thread looks for its next one, which comes after it in the order.
+// The k largest of n candidates at(i) to out[0..k) (0 where they run out). The k-th best of what groups of four threads have is a bound: what is at
+// least as good lies in k groups, which look through their shares again and put it on a list, whose entries then count who is in front of them.
+// (Rounds of one maximum each took 24 us for 20 of 1000 segments and 20 of 2560 values; ranks of all 256 threads' bests 18.) The list holds LIST
+// entries: n up to LIST / (4 k) x THREADS; more candidates are picked in rounds.
+constexpr int GROUP = 4, GROUPS = THREADS / GROUP, LIST = 4096;
+static_assert(GROUPS >= LOGPROBS_MAX_TOP, "the bound is one group's");
+struct Select {
+    Key best[GROUPS], list[LIST], bound;
+    int n;
+};
+__device__ __forceinline__ bool select_takes(int64_t n, int k) { return (n + THREADS - 1) / THREADS * GROUP * k <= LIST; }
 template <typename F>
-__device__ __forceinline__ void pick(int n, int k, const F &at, Best *out, Best (*sh)[WARPS]) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Best last = {INT32_MAX, 0};
-    auto next = [&]() {
-        Best b = {NONE, 0xffffffffu};
+__device__ __forceinline__ void select(int n, int k, const F &at, Key *out, Select &sh) {
+    Key mine = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += THREADS) mine = max(mine, at(i));
+    Key group = max(mine, (Key)__shfl_xor_sync(0xffffffffu, mine, 1));
+    group = max(group, (Key)__shfl_xor_sync(0xffffffffu, group, 2));
+    if (threadIdx.x % GROUP == 0) sh.best[threadIdx.x / GROUP] = group;
+    if (threadIdx.x == 0) {
+        sh.bound = 1;   // fewer than k groups have any: all candidates
+        sh.n = 0;
+    }
+    if (threadIdx.x < k) out[threadIdx.x] = 0;
+    __syncthreads();
+    if (threadIdx.x < GROUPS) {
+        const Key b = sh.best[threadIdx.x];
+        int ahead = 0;
+#pragma unroll 16
+        for (int i = 0; i < GROUPS; i++) ahead += sh.best[i] > b;
+        if (ahead == k - 1 && b) sh.bound = b;
+    }
+    __syncthreads();
+    const Key bound = sh.bound;
+    if (mine >= bound) {
+#pragma unroll 4
         for (int i = threadIdx.x; i < n; i += THREADS) {
-            const Best c = at(i);
-            if (c.o > NONE && after(c.o, c.id, last) && (c.o > b.o || (c.o == b.o && c.id < b.id))) b = c;
+            const Key c = at(i);
+            if (c >= bound) sh.list[atomicAdd(&sh.n, 1)] = c;
+        }
+    }
+    __syncthreads();
+    const int listed = sh.n;
+    for (int i = threadIdx.x; i < listed; i += THREADS) {
+        const Key c = sh.list[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < listed; j++) rank += sh.list[j] > c;
+        if (rank < k) out[rank] = c;
+    }
+    __syncthreads();
+}
+// The same in rounds, for any number of candidates: every thread keeps the best of its share behind the last one picked.
+template <typename F>
+__device__ __forceinline__ void pick(int n, int k, const F &at, Key *out, Key (*sh)[WARPS]) {
+    Key last = ~0ull;
+    auto next = [&]() {
+        Key b = 0;
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+            const Key c = at(i);
+            if (c < last) b = max(b, c);
         }
         return b;
     };
-    Best mine = next();
+    Key mine = next();
     for (int r = 0; r < k; r++) {
-        const int o = __reduce_max_sync(0xffffffffu, mine.o);
-        const uint32_t id = __reduce_min_sync(0xffffffffu, mine.o == o ? mine.id : 0xffffffffu);
-        if (lane == 0) sh[r & 1][warp] = {o, id};
-        __syncthreads();
-        Best w = sh[r & 1][0];
+        Key w = mine;
 #pragma unroll
-        for (int i = 1; i < WARPS; i++) {
-            const Best c = sh[r & 1][i];
-            if (c.o > w.o || (c.o == w.o && c.id < w.id)) w = c;
-        }
+        for (int o = 16; o > 0; o >>= 1) w = max(w, (Key)__shfl_xor_sync(0xffffffffu, w, o));
+        if ((threadIdx.x & 31) == 0) sh[r & 1][threadIdx.x >> 5] = w;
+        __syncthreads();
+        w = sh[r & 1][0];
+#pragma unroll
+        for (int i = 1; i < WARPS; i++) w = max(w, sh[r & 1][i]);
         if (threadIdx.x == 0) out[r] = w;
-        if (w.id == 0xffffffffu) {
-            for (int j = r + 1 + (int)threadIdx.x; j < k; j += THREADS) out[j] = w;
-            break;
-        }
-        if (mine.id == w.id) {
-            last = mine;
+        if (w && mine == w) {
+            last = w;
             mine = next();
         }
     }
     __syncthreads();
 }
-// -inf and what the order puts below it are no candidates
-__device__ __forceinline__ int candidate(float x) { return x > -CUDART_INF_F ? order(x) : NONE; }
 }  // namespace lp
 
 template <typename T>
@@ -209,52 +307,64 @@ __global__ void __launch_bounds__(lp::THREADS) k_logprobs_finish(const __grid_co
     constexpr int SEG = Vec<T>::SEG;
     griddep_launch();
     griddep_wait();
-    __shared__ Sums sh[WARPS];
-    __shared__ Best bsh[2][WARPS], segs[LOGPROBS_MAX_TOP], best[LOGPROBS_MAX_TOP];
+    __shared__ Sums row_s;
+    __shared__ float log_s_s;
+    __shared__ Key rounds[2][WARPS], segs[LOGPROBS_MAX_TOP], best[LOGPROBS_MAX_TOP];
+    __shared__ Select sel;
     const int64_t row_i = blockIdx.x;
     const Logprobs &a = p.a;
     const T *row = reinterpret_cast<const T *>((const char *)a.logits + row_i * a.stride);
-    Sums v = {-CUDART_INF_F, 0.f, 0.f};
-    for (int i = threadIdx.x; i < p.splits; i += THREADS) v = join(v, p.part[row_i * p.splits + i]);
-    v = join_block(v, sh);
-    const bool undefined = !(v.s == v.s), empty = v.s == 0.f;   // a NaN or +inf among the logits; nothing but -inf
-    const float log_s = logf(v.s);
-    if (threadIdx.x == 0) {
-        if (a.logprob) {
-            const int32_t tok = a.tokens ? a.tokens[row_i] : -1;
-            float y = 0.f;
-            if (tok >= 0 && tok < a.vocab) {
-                y = undefined ? CUDART_NAN_F : (empty ? -CUDART_INF_F : (value(row[tok]) - v.m) - log_s);
-            } else if (tok != -1) {
-                y = CUDART_NAN_F;
-                if (a.err) report_error(a.err, TLB_ERR_INDEX);
-            }
-            a.logprob[row_i * a.out_step] = y;
+    if (threadIdx.x < 32) {   // the other warps begin to look for the alternatives
+        Sums v = {-CUDART_INF_F, 0.f, 0.f};
+        for (int i = threadIdx.x; i < p.splits; i += 32) {
+            Sums w = p.part[row_i * p.splits + i];
+            const float m = fmaxf(v.m, w.m);
+            move_to(v, m);
+            move_to(w, m);
+            v.s += w.s;
+            v.t += w.t;
         }
-        if (a.entropy) a.entropy[row_i * a.out_step] = undefined ? CUDART_NAN_F : (empty ? 0.f : log_s - v.t / v.s);
+        v = join_warp(v);
+        const bool undefined = !(v.s == v.s), empty = v.s == 0.f;   // a NaN or +inf among the logits; nothing but -inf
+        const float log_s = logf(v.s);
+        if (threadIdx.x == 0) {
+            row_s = v;
+            log_s_s = log_s;
+            if (a.logprob) {
+                const int32_t tok = a.tokens ? a.tokens[row_i] : -1;
+                float y = 0.f;
+                if (tok >= 0 && tok < a.vocab) {
+                    y = undefined ? CUDART_NAN_F : (empty ? -CUDART_INF_F : (value(row[tok]) - v.m) - log_s);
+                } else if (tok != -1) {
+                    y = CUDART_NAN_F;
+                    if (a.err) report_error(a.err, TLB_ERR_INDEX);
+                }
+                a.logprob[row_i * a.out_step] = y;
+            }
+            if (a.entropy) a.entropy[row_i * a.out_step] = undefined ? CUDART_NAN_F : (empty ? 0.f : log_s - v.t / v.s);
+        }
     }
     if (a.top == 0) return;
-    if (!undefined && !empty) {
-        const float *seg_max = p.seg_max + row_i * p.segs;
-        const int shift = shift_of(row);
-        pick(p.segs, a.top, [&](int i) { return Best{candidate(seg_max[i]), (uint32_t)i}; }, segs, bsh);
-        pick(a.top * SEG, a.top, [&](int i) {
-            const uint32_t seg = segs[i / SEG].id;
-            const int64_t id = (int64_t)seg * SEG + i % SEG - shift;
-            if (seg == 0xffffffffu || id < 0 || id >= a.vocab) return Best{NONE, 0xffffffffu};
-            return Best{candidate(value(row[id])), (uint32_t)id};
-        }, best, bsh);
-    } else {
-        if (threadIdx.x < a.top) best[threadIdx.x] = {NONE, 0xffffffffu};
-        __syncthreads();
-    }
+    const float *seg_max = p.seg_max + row_i * p.turns * UNROLL;
+    const int shift = shift_of(row), n = p.turns * UNROLL;
+    const auto segment = [&](int i) { return key_of(seg_max[i], (uint32_t)i); };
+    if (select_takes(n, a.top)) select(n, a.top, segment, segs, sel);
+    else pick(n, a.top, segment, segs, rounds);
+    static_assert(LOGPROBS_MAX_TOP * 256 / THREADS * GROUP * LOGPROBS_MAX_TOP <= LIST, "the values of the segments always fit the list");
+    select(a.top * SEG, a.top, [&](int i) -> Key {
+        const Key seg = segs[i / SEG];
+        const int64_t id = (int64_t)id_of(seg) * SEG + i % SEG - shift;
+        return seg && id >= 0 && id < a.vocab ? key_of(value(row[id]), (uint32_t)id) : 0;
+    }, best, sel);
     if (threadIdx.x < a.top) {
-        const Best b = best[threadIdx.x];
-        const bool none = b.id == 0xffffffffu;
+        const Sums v = row_s;
+        const bool undefined = !(v.s == v.s);
+        const float log_s = log_s_s;
+        const Key b = undefined ? 0 : best[threadIdx.x];
         const int64_t at = row_i * a.top_step + threadIdx.x;
-        if (a.ids_f32) ((float *)a.top_ids)[at] = none ? -1.f : (float)b.id;
-        else ((int32_t *)a.top_ids)[at] = none ? -1 : (int32_t)b.id;
-        a.top_logprobs[at] = undefined ? CUDART_NAN_F : (none ? -CUDART_INF_F : (unorder(b.o) - v.m) - log_s);
+        if (a.ids_f32) ((float *)a.top_ids)[at] = b ? (float)id_of(b) : -1.f;
+        else ((int32_t *)a.top_ids)[at] = b ? (int32_t)id_of(b) : -1;
+        a.top_logprobs[at] = undefined ? CUDART_NAN_F : (b ? (value_of(b) - v.m) - log_s : -CUDART_INF_F);
     }
 }
 
@@ -263,12 +373,16 @@ template <typename T>
 static lp::Scan lp_plan(const Logprobs &a, int sm_count, uint64_t *bytes) {
     lp::Scan p{};
     p.a = a;
-    p.segs = (int)((a.vocab + lp::Vec<T>::N - 1 + lp::Vec<T>::SEG - 1) / lp::Vec<T>::SEG);   // wherever in 16 bytes a row starts
-    const int64_t most = std::min<int64_t>(256, (p.segs + lp::WARPS - 1) / lp::WARPS);
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, (sm_count * 32 + a.rows - 1) / std::max<int64_t>(a.rows, 1)));
-    p.segs_per_split = (p.segs + p.splits - 1) / p.splits;
-    p.splits = std::max(1, (p.segs + p.segs_per_split - 1) / p.segs_per_split);
-    *bytes = ((uint64_t)a.rows * p.splits * sizeof(lp::Sums) + 15) / 16 * 16 + (a.top ? (uint64_t)a.rows * p.segs * 4 : 0);
+    constexpr int64_t TURN = (int64_t)lp::Vec<T>::SEG * lp::UNROLL;
+    p.turns = (int)((a.vocab + lp::Vec<T>::N - 1 + TURN - 1) / TURN);   // wherever in 16 bytes a row starts
+    // Eight turns of every warp where there are rows enough for 24 CTAs per SM, down to one; with few rows, CTAs of fewer warps' turns
+    int64_t per = 8 * lp::WARPS;
+    const auto ctas = [&](int64_t n) { return a.rows * ((p.turns + n - 1) / n); };
+    while (per > lp::WARPS && ctas(per) < (int64_t)sm_count * 24) per /= 2;
+    while (per > 2 && ctas(per) < sm_count) per /= 2;
+    p.turns_per_split = (int)std::max<int64_t>(per, (p.turns + 255) / 256);
+    p.splits = (p.turns + p.turns_per_split - 1) / p.turns_per_split;
+    *bytes = ((uint64_t)a.rows * p.splits * sizeof(lp::Sums) + 15) / 16 * 16 + (a.top ? (uint64_t)a.rows * p.turns * lp::UNROLL * 4 : 0);
     return p;
 }
 template <typename T>

@@ -41,7 +41,7 @@ cudaError_t tc_encode_sw128(CUtensorMap *map, const void *base, int rank, const 
 
 namespace sat {
 constexpr int T = 128;
-constexpr int THREADS = 384;            // warp 0 copies, warp 1 issues MMAs, warps 2-3 look through special tiles, 4-7 and 8-11 the streams
+constexpr int THREADS = 384;            // warp 0 shares out the work and copies queries and keys, 3 values, 1 issues MMAs, 2 looks through special tiles, 4-7 and 8-11 are the streams
 constexpr int HALF_BYTES = T * 128;     // 128 rows of 64 elements
 constexpr float RESCALE_STEP = 8.f;     // in the base-2 domain
 constexpr uint32_t O_COL = 256;         // S / P of stream x at column 128 x, O at 256 + 128 x
@@ -53,6 +53,10 @@ __host__ __device__ constexpr int stages(int hsp, bool share) { return hsp == 12
 __host__ __device__ constexpr int tile_bytes(int hsp) { return T * hsp * 2; }
 __host__ __device__ constexpr int smem_bytes(int hsp, bool share) { return ((share ? 2 : 1) + 2 * stages(hsp, share)) * tile_bytes(hsp); }
 
+struct Place {
+    int seq, kvh, r;
+    int64_t off;    // units of this row tile in front of the place
+};
 struct Params {
     CUtensorMap q, k, v;
     ServeAttn a;
@@ -60,6 +64,7 @@ struct Params {
     int group, tpt, tt;       // heads per KV head; tokens of a row tile; of the row tiles that a unit covers
     int ctas, min_units;      // a CTA's least share
     int pool_rows;            // paged: rows of a pool
+    Place *ends;              // [CTA]: where its stretch ends, which tells k_serve_join what it cuts
     float *partial;           // [CTA][2]: (m, l) of the rows, then O as [hsp / 4][rows][4], which the writers' lanes (rows) fill side by side
 };
 
@@ -107,10 +112,9 @@ __device__ __forceinline__ int64_t units_before(const Params &p, const ServeSeq 
     if (r == R && R > 0) u += key_tiles<false>(p, s, R - 1);
     return u;
 }
-struct Place {
-    int seq, kvh, r;
-    int64_t off;    // units of this row tile in front of the place
-};
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {   // of numbers that are not negative; 64-bit division takes ten times as long
+    return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
 // By one warp: the number of all units, and the place of one
 template <bool PAGED>
 __device__ __forceinline__ int64_t seq_units(const Params &p, int s) {
@@ -145,8 +149,8 @@ __device__ __forceinline__ Place find_unit(const Params &p, int64_t at, int64_t 
             Place w;
             w.seq = s0 + l;
             at -= __shfl_sync(0xffffffffu, upto - u, l);
-            const int64_t head = __shfl_sync(0xffffffffu, u, l) / p.a.kv_heads;
-            w.kvh = (int)(at / head);
+            const int64_t head = divide(__shfl_sync(0xffffffffu, u, l), p.a.kv_heads);
+            w.kvh = (int)divide(at, head);
             at -= w.kvh * head;
             // the last row tile that starts at or before `at`: 32 places at a time
             const ServeSeq q = serve_seq(p.a, w.seq);
@@ -168,7 +172,7 @@ __device__ __forceinline__ Place find_unit(const Params &p, int64_t at, int64_t 
     }
     return {p.a.seqs, 0, 0, 0};
 }
-__device__ __forceinline__ int64_t share_of(const Params &p, int64_t total) { return max((int64_t)p.min_units, (total + p.ctas - 1) / p.ctas); }
+__device__ __forceinline__ int64_t share_of(const Params &p, int64_t total) { return max((int64_t)p.min_units, divide(total + p.ctas - 1, p.ctas)); }
 
 // A stretch of the key tiles of one row tile, as the copying warp tells it to the others
 struct Segment {
@@ -457,7 +461,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             mbar_init(&bar_kfree[i], 1);
             mbar_init(&bar_v[i], 1);
             mbar_init(&bar_vfree[i], 1);
-            mbar_init(&bar_fix[i], 2);
+            mbar_init(&bar_fix[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&bar_s[i], 1);
@@ -495,6 +499,40 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         return g.t0 >= 0 && !*fail;
     };
 
+    // The tiles of a segment on their way to a ring of stages (warp 0: keys, warp 3: values), in front of each `before(tile)`
+    auto copy_tiles = [&](uint8_t *ring, const CUtensorMap *map, uint64_t *full, uint64_t *free, int &tile, auto &&before) {
+        // paged: a box per page and 64 columns. The page's row in the pool is looked up a tile ahead, by a lane each; pages that are not needed
+        // and bad ids lie past the pool: zeros. One lane issues (a warp's lanes one after another took 72 cycles per box).
+        const int rows = min(p.a.block_size, T), boxes = T / rows;   // 1 to 16 pages
+        auto page_row = [&](int j) {
+            const int key = j * T + lane * rows;
+            if (lane >= boxes || key >= g.nk || j >= g.t1) return p.pool_rows;
+            const int32_t blk = p.a.tables[(int64_t)g.seq * p.a.max_blocks + key / p.a.block_size];
+            if (blk >= 0 && blk < p.a.pool_blocks) return (blk * p.a.kv_heads + g.kvh) * p.a.block_size + key % p.a.block_size;
+            if (p.a.err) report_error(p.a.err, TLB_ERR_INDEX);
+            return p.pool_rows;
+        };
+        int row = PAGED ? page_row(g.t0) : 0;
+        for (int j = g.t0; j < g.t1; j++, tile++) {
+            before(j);
+            const int ahead = PAGED ? page_row(j + 1) : 0, s = tile % NS;
+            mbar_wait_nap(&free[s], (uint32_t)(tile / NS + 1) & 1u, fail, 32);
+            if (__any_sync(0xffffffffu, *fail)) return;
+            if (lane == 0) mbar_expect_tx(&full[s], TILE);
+            if (!PAGED) {
+                if (lane == 0)
+                    for (int h = 0; h < HALVES; h++) tma_3d(ring + s * TILE + h * HALF_BYTES, map, h * 64, g.kvh, g.k0 + j * T, &full[s]);
+            } else {
+#pragma unroll 4
+                for (int b = 0; b < boxes; b++) {
+                    const int r = __shfl_sync(0xffffffffu, row, b);
+                    if (lane == 0)
+                        for (int h = 0; h < HALVES; h++) tma_2d(ring + s * TILE + h * HALF_BYTES + b * rows * 128, map, h * 64, r, &full[s]);
+                }
+            }
+            row = ahead;
+        }
+    };
     if (warp == 0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
         // ---- copies. The keys of a segment's first tiles are on their way before its queries, whose room the segment in front still uses.
@@ -502,8 +540,9 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         {
             int64_t seq0;
             const int64_t total = total_units<PAGED>(p, seq0), share = share_of(p, total), first = share * blockIdx.x;
+            if (lane == 0 && blockIdx.x == 0) p.ends[p.ctas].off = share;
             walk.left = min(share, total - first);
-            if (walk.left > 0) walk.at = find_unit<PAGED>(p, first, seq0);
+            walk.at = walk.left > 0 ? find_unit<PAGED>(p, first, seq0) : Place{p.a.seqs, 0, 0, 0};
         }
         auto tell = [&]() {
             const int r = g_at % SEG_RING;
@@ -529,45 +568,9 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 }
                 have_q = true;
             };
-            for (int j = g.t0; j < g.t1; j++, tile++) {
+            copy_tiles(ks, &p.k, bar_k, bar_kfree, tile, [&](int j) {
                 if (!have_q && (j - g.t0 >= NS || __any_sync(0xffffffffu, mbar_test(su32(&bar_qfree), (uint32_t)(seg + 1) & 1u)))) load_q();
-                const int s = tile % NS;
-                const uint32_t free_parity = (uint32_t)(tile / NS + 1) & 1u;
-                if (!PAGED) {
-                    if (lane == 0) {
-                        const int z = g.k0 + j * T;
-                        mbar_wait_nap(&bar_kfree[s], free_parity, fail, 32);
-                        mbar_expect_tx(&bar_k[s], TILE);
-                        for (int h = 0; h < HALVES; h++) tma_3d(ks + s * TILE + h * HALF_BYTES, &p.k, h * 64, g.kvh, z, &bar_k[s]);
-                        mbar_wait_nap(&bar_vfree[s], free_parity, fail, 32);
-                        mbar_expect_tx(&bar_v[s], TILE);
-                        for (int h = 0; h < HALVES; h++) tma_3d(vs + s * TILE + h * HALF_BYTES, &p.v, h * 64, g.kvh, z, &bar_v[s]);
-                    }
-                } else {
-                    // a box per page and 64 columns, a lane each; pages that are not needed and bad ids lie past the pool: zeros
-                    const int rows = min(p.a.block_size, T), boxes = T / rows;   // 1 to 16 pages
-                    int row = p.pool_rows;
-                    if (lane < boxes) {
-                        const int key = j * T + lane * rows;
-                        if (key < g.nk) {
-                            const int32_t blk = p.a.tables[(int64_t)g.seq * p.a.max_blocks + key / p.a.block_size];
-                            if (blk >= 0 && blk < p.a.pool_blocks) row = (blk * p.a.kv_heads + g.kvh) * p.a.block_size + key % p.a.block_size;
-                            else if (p.a.err) report_error(p.a.err, TLB_ERR_INDEX);
-                        }
-                    }
-                    row = __shfl_sync(0xffffffffu, row, lane % boxes);
-                    const int h = lane / boxes, dst = h * HALF_BYTES + lane % boxes * rows * 128;
-                    mbar_wait_nap(&bar_kfree[s], free_parity, fail, 32);
-                    if (lane == 0) mbar_expect_tx(&bar_k[s], TILE);
-                    __syncwarp();
-                    if (h < HALVES) tma_2d(ks + s * TILE + dst, &p.k, h * 64, row, &bar_k[s]);
-                    mbar_wait_nap(&bar_vfree[s], free_parity, fail, 32);
-                    if (lane == 0) mbar_expect_tx(&bar_v[s], TILE);
-                    __syncwarp();
-                    if (h < HALVES) tma_2d(vs + s * TILE + dst, &p.v, h * 64, row, &bar_v[s]);
-                }
-                if (__any_sync(0xffffffffu, *fail)) break;
-            }
+            });
             if (__any_sync(0xffffffffu, *fail)) break;
             if (!have_q) load_q();
             __syncwarp();
@@ -575,16 +578,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         }
         g.t0 = -1;
         tell();
-        // only after a wait has given up: this CTA's copies are over before its shared memory is
-        if (*fail && lane == 0) {
-            mbar_wait_limit(&bar_q, 0, 1u << 12);
-            for (int i = 0; i < NS; i++) {
-                mbar_wait_limit(&bar_k[i], 0, 1u << 10);
-                mbar_wait_limit(&bar_k[i], 1, 1u << 10);
-                mbar_wait_limit(&bar_v[i], 0, 1u << 10);
-                mbar_wait_limit(&bar_v[i], 1, 1u << 10);
-            }
-        }
+        if (lane == 0) p.ends[blockIdx.x] = walk.left == 0 ? walk.at : Place{p.a.seqs, 0, 0, 0};
     } else if (warp == 1) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
         // ---- MMA issue: step i is stream i & 1; S of step i + 2 follows O of step i, which has read the P that it overwrites
@@ -634,7 +628,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             tile += n;
             seg++;
         }
-    } else if (warp < 4) {
+    } else if (warp == 2) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
         // ---- every tile of values passes here, in order, on its way to the MMAs. Special ones: rows behind the end become zero, the others are
         // looked through
@@ -650,7 +644,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                     constexpr uint32_t EXP = BF16 ? 0x7f807f80u : 0x7c007c00u;
                     uint32_t odd = 0;
 #pragma unroll 8
-                    for (int i = tid - 64; i < TILE / 16; i += 64) {
+                    for (int i = lane; i < TILE / 16; i += 32) {
                         if (((i >> 3) & (T - 1)) >= live) {
                             v[i] = make_uint4(0, 0, 0, 0);
                         } else {
@@ -666,6 +660,10 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             }
             seg++;
         }
+    } else if (warp == 3) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
+        int tile = 0;
+        while (next()) copy_tiles(vs, &p.v, bar_v, bar_vfree, tile, [](int) {});
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_STREAMS));
         // ---- the streams
@@ -850,6 +848,14 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             seg++;
         }
     }
+    // only after a wait has given up: this CTA's copies are over before its shared memory is
+    if (*fail && tid == 0) {
+        mbar_wait_limit(&bar_q, 0, 1u << 12);
+        for (int i = 0; i < 2 * NS; i++) {
+            mbar_wait_limit(&bar_k[i >> 1], i & 1, 1u << 10);
+            mbar_wait_limit(&bar_v[i >> 1], i & 1, 1u << 10);
+        }
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == 0) tmem_dealloc(tmem, 512);
@@ -863,25 +869,15 @@ __global__ void __launch_bounds__(128) k_serve_join(const __grid_constant__ sat:
     constexpr int NQ = SHARE ? 2 : 1, ROWS = NQ * T, SLOT = ROWS * (2 + HSP);
     griddep_launch();
     griddep_wait();
-    __shared__ Place at_s;
-    __shared__ int64_t share_s;
     const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) {
-        int64_t seq0;
-        const int64_t total = total_units<PAGED>(p, seq0), share = share_of(p, total), end = share * (c + 1);
-        const Place w = end < total ? find_unit<PAGED>(p, end, seq0) : Place{p.a.seqs, 0, 0, 0};
-        if (lane == 0) {
-            at_s = w;
-            share_s = share;
-        }
-    }
-    __syncthreads();
-    const Place w = at_s;
-    if (w.seq >= p.a.seqs || w.off == 0 || w.off > share_s) return;   // nothing begins here, or in a stretch in front
+    const Place w = p.ends[c];
+    if (w.seq >= p.a.seqs || w.off == 0) return;   // nothing is cut here
+    const Place v = c ? p.ends[c - 1] : Place{0, 0, 0, 0};
+    if (v.off > 0 && v.seq == w.seq && v.kvh == w.kvh && v.r == w.r) return;   // it begins in a stretch in front
     const ServeSeq sq = serve_seq(p.a, w.seq);
     const int n = key_tiles<PAGED>(p, sq, w.r);
     if (w.off >= n) return;   // all of its key tiles lie in this stretch
-    const int parts = 1 + (int)((n - w.off + share_s - 1) / share_s);
+    const int parts = 1 + (int)((n - w.off + p.ends[p.ctas].off - 1) / p.ends[p.ctas].off);
     // 32 rows: a lane's row is its own, a warp's columns a quarter of them
     const int row = blockIdx.y * 32 + lane, x = row / T, rr = row % T;
     const int token = w.r * p.tt + x * p.tpt + rr / p.group, head = w.kvh * p.group + rr % p.group;
@@ -938,8 +934,10 @@ static int sat_ctas(const ServeAttn &a, int sm_count) {
     const double units = (double)tiles * a.kv_heads * (double)(keys + sat::OVERHEAD);
     return units / 2 < sm_count ? std::max(1, (int)(units / 2 + 1)) : sm_count;
 }
+static uint64_t sat_ends_bytes(int ctas) { return ((uint64_t)(ctas + 1) * sizeof(sat::Place) + 255) / 256 * 256; }   // the last one: the size of a share
 uint64_t serve_attn_tc_scratch_bytes(const ServeAttn &a, int sm_count) {
-    return (uint64_t)sat_ctas(a, sm_count) * 2 * (sat_share(a) ? 2 : 1) * sat::T * (2 + (a.hs <= 64 ? 64 : 128)) * 4;
+    const uint64_t ctas = (uint64_t)sat_ctas(a, sm_count);
+    return sat_ends_bytes((int)ctas) + ctas * 2 * (sat_share(a) ? 2 : 1) * sat::T * (2 + (a.hs <= 64 ? 64 : 128)) * 4;
 }
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
 static cudaError_t sat_launch(const sat::Params &p, int ctas, cudaStream_t st) {
@@ -976,7 +974,6 @@ cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count
     const bool share = sat_share(a);
     p.tt = p.tpt * (share ? 2 : 1);
     p.min_units = 1 + OVERHEAD;
-    p.partial = (float *)scratch;
     const uint64_t hs = (uint64_t)a.hs;
     cudaError_t e;
     {
@@ -998,6 +995,8 @@ cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count
     }
     if (e != cudaSuccess) return e;
     const int ctas = p.ctas = sat_ctas(a, sm_count);
+    p.ends = (Place *)scratch;
+    p.partial = (float *)((char *)scratch + sat_ends_bytes(ctas));
     if (a.paged) return a.hs <= 64 ? sat_launch<64, false, true, false>(p, ctas, st) : sat_launch<128, false, true, false>(p, ctas, st);
     if (a.hs <= 64) {
         if (a.bf16) return share ? sat_launch<64, true, false, true>(p, ctas, st) : sat_launch<64, true, false, false>(p, ctas, st);

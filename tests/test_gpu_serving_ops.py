@@ -393,7 +393,7 @@ def check_logprobs(got, want, x):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 2, 5), (2, 31, 31), (5, 127, 20), (1, 129, 32), (4, 1000, 0), (7, 4097, 1), (2, 32001, 20), (1, 128256, 20), (40, 5003, 8), (2, 300007, 32)])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 2, 5), (2, 31, 31), (5, 127, 20), (1, 129, 32), (4, 1000, 0), (7, 4097, 1), (2, 32001, 20), (1, 128256, 20), (40, 5003, 8), (2, 300007, 32), (1, 1300001, 32)])
 def test_token_logprobs(native, dtype, rows, vocab, top):
     """Odd vocabularies put the rows of 16-bit logits off 16 bytes; bf16 has many equal logits."""
     x = randn((rows, vocab), rows + vocab, torch.float32)
