@@ -130,6 +130,10 @@ def test_arrays_of_the_wrong_kind_are_refused():
     refused("kv heads, head size", go, q, k, k, at, array(3, (9, 4, 64), "<f2"))
     refused("sequences + 1", go, q, k, k, array(2, (0,), "<i4"), out)
     refused("kv_offsets", go, q, k, k, at, out, kv_offsets=array(4, (4,), "<i4"))
+    wide = array(0, (1, 2 ** 33, 64), "<f2")
+    refused("out of range", go, wide, k, k, at, wide)
+    refused("not an array", go, q, k, None, at, out)
+    refused("whole elements", go, array(0, (10, 4, 64), "<f2", (513, 128, 2)), k, k, at, out)
     refused("status", go, q, k, k, at, out, status=array(4, (2,), "<i4"))
     x = array(0, (5, 100), "<f4")
     refused("shape", ops.token_logprobs, x, array(1, (4,), "<i4"), array(2, (5,), "<f4"))
