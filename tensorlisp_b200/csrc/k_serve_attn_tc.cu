@@ -42,16 +42,16 @@ cudaError_t tc_encode_sw128(CUtensorMap *map, const void *base, int rank, const 
 namespace sat {
 constexpr int T = 128;
 constexpr int THREADS = 384;            // warp 0 shares out the work and copies queries and keys, 3 values, 1 issues MMAs, 2 looks through special tiles, 4-7 and 8-11 are the streams
-constexpr int HALF_BYTES = T * 128;     // 128 rows of 64 elements
 constexpr float RESCALE_STEP = 8.f;     // in the base-2 domain
 constexpr uint32_t O_COL = 256;         // S / P of stream x at column 128 x, O at 256 + 128 x
 constexpr int SLOW_RING = 16;
 constexpr int REGS_ROLES = 88, REGS_STREAMS = 200;   // registers of a thread (setmaxnreg): the streams hold a row of 128 scores
 constexpr int OVERHEAD = 2;             // what a row tile costs beside its key tiles, in key tiles
 
-__host__ __device__ constexpr int stages(int hsp, bool share) { return hsp == 128 ? (share ? 2 : 3) : (share ? 4 : 6); }
-__host__ __device__ constexpr int tile_bytes(int hsp) { return T * hsp * 2; }
-__host__ __device__ constexpr int smem_bytes(int hsp, bool share) { return ((share ? 2 : 1) + 2 * stages(hsp, share)) * tile_bytes(hsp); }
+// Keys of a tile. 64 without SHARE: a tile of values is held for a shorter time and more of them are on their way in the same room
+__host__ __device__ constexpr int key_tile(bool share) { return share ? 128 : 64; }
+__host__ __device__ constexpr int stages(int hsp, bool share) { return hsp == 128 ? (share ? 2 : 6) : (share ? 4 : 8); }
+__host__ __device__ constexpr int smem_bytes(int hsp, bool share) { return ((share ? 2 : 1) * T + 2 * stages(hsp, share) * key_tile(share)) * hsp * 2; }
 
 struct Place {
     int seq, kvh, r;
@@ -61,9 +61,9 @@ struct Params {
     CUtensorMap q, k, v;
     ServeAttn a;
     float scale_log2;
+    int pool_rows;            // paged: rows of a pool
     int group, tpt, tt;       // heads per KV head; tokens of a row tile; of the row tiles that a unit covers
     int ctas, min_units;      // a CTA's least share
-    int pool_rows;            // paged: rows of a pool
     Place *ends;              // [CTA]: where its stretch ends, which tells k_serve_join what it cuts
     float *partial;           // [CTA][2]: (m, l) of the rows, then O as [hsp / 4][rows][4], which the writers' lanes (rows) fill side by side
 };
@@ -90,54 +90,63 @@ __device__ __forceinline__ int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a,
 template <bool PAGED>
 __device__ __forceinline__ int row_tiles(const Params &p, const ServeSeq &s) { return ((PAGED ? p.a.drafts : s.nq) + p.tt - 1) / p.tt; }
 // key tiles of row tile r
-template <bool PAGED>
+template <bool PAGED, int KT>
 __device__ __forceinline__ int key_tiles(const Params &p, const ServeSeq &s, int r) {
-    if (PAGED) return r * p.tt < s.nq ? (int)((s.nk + T - 1) / T) : 0;
+    if (PAGED) return r * p.tt < s.nq ? (int)((s.nk + KT - 1) / KT) : 0;
     const int64_t last = min((int64_t)s.nq, (int64_t)(r + 1) * p.tt) - 1 + s.nk - s.nq;   // the last key that its last token sees
-    return last < 0 ? 0 : (int)(last / T) + 1;
+    return last < 0 ? 0 : (int)(last / KT) + 1;
 }
 // units of row tiles [0, r)
-template <bool PAGED>
+template <bool PAGED, int KT>
 __device__ __forceinline__ int64_t units_before(const Params &p, const ServeSeq &s, int r) {
     int64_t u = (int64_t)r * OVERHEAD;
-    if (PAGED) return u + (int64_t)min(r, (s.nq + p.tt - 1) / p.tt) * ((s.nk + T - 1) / T);
+    if (PAGED) return u + (int64_t)min(r, (s.nq + p.tt - 1) / p.tt) * ((s.nk + KT - 1) / KT);
     const int R = row_tiles<false>(p, s);
     const int full = min(r, R - 1);
     const int64_t off = s.nk - s.nq;
     const int first = off < 0 ? (int)min((int64_t)full, -off / p.tt) : 0;   // row tiles that see nothing
-    if (full > first) {   // floor((off + (i + 1) tt - 1) / T) + 1 of the tiles in between; whole key tiles of off go in front
-        const int64_t b = off + (int64_t)(first + 1) * p.tt - 1 + T;
-        u += (int64_t)(full - first) * (b / T) + floor_sum((uint32_t)(full - first), T, (uint32_t)p.tt, (uint32_t)(b % T));
+    if (full > first) {   // floor((off + (i + 1) tt - 1) / KT) + 1 of the tiles in between; whole key tiles of off go in front
+        const int64_t b = off + (int64_t)(first + 1) * p.tt - 1 + KT;
+        u += (int64_t)(full - first) * (b / KT) + floor_sum((uint32_t)(full - first), KT, (uint32_t)p.tt, (uint32_t)(b % KT));
     }
-    if (r == R && R > 0) u += key_tiles<false>(p, s, R - 1);
+    if (r == R && R > 0) u += key_tiles<false, KT>(p, s, R - 1);
     return u;
 }
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {   // of numbers that are not negative; 64-bit division takes ten times as long
     return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 // By one warp: the number of all units, and the place of one
-template <bool PAGED>
-__device__ __forceinline__ int64_t seq_units(const Params &p, int s) {
-    if (s >= p.a.seqs) return 0;
-    const ServeSeq q = serve_seq(p.a, s);
-    return units_before<PAGED>(p, q, row_tiles<PAGED>(p, q)) * p.a.kv_heads;
+struct LaneSeq {
+    ServeSeq q;
+    int64_t units;
+};
+template <bool PAGED, int KT>
+__device__ __forceinline__ LaneSeq lane_seq(const Params &p, int s) {
+    LaneSeq r;
+    r.units = 0;
+    if (s < p.a.seqs) {
+        r.q = serve_seq(p.a, s);
+        r.units = units_before<PAGED, KT>(p, r.q, row_tiles<PAGED>(p, r.q)) * p.a.kv_heads;
+    }
+    return r;
 }
-// first: the units of sequence `lane`, which find_unit begins with
-template <bool PAGED>
-__device__ __forceinline__ int64_t total_units(const Params &p, int64_t &first) {
+// first: sequence `lane`, with which find_unit begins
+template <bool PAGED, int KT>
+__device__ __forceinline__ int64_t total_units(const Params &p, LaneSeq &first) {
     const int lane = threadIdx.x & 31;
-    int64_t u = first = seq_units<PAGED>(p, lane);
-    for (int s = lane + 32; s < p.a.seqs; s += 32) u += seq_units<PAGED>(p, s);
+    first = lane_seq<PAGED, KT>(p, lane);
+    int64_t u = first.units;
+    for (int s = lane + 32; s < p.a.seqs; s += 32) u += lane_seq<PAGED, KT>(p, s).units;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
     return u;
 }
-template <bool PAGED>
-__device__ __forceinline__ Place find_unit(const Params &p, int64_t at, int64_t first) {
+template <bool PAGED, int KT>
+__device__ __forceinline__ Place find_unit(const Params &p, int64_t at, const LaneSeq &first, ServeSeq &q) {
     const int lane = threadIdx.x & 31;
     for (int s0 = 0; s0 < p.a.seqs; s0 += 32) {
-        const int64_t u = s0 ? seq_units<PAGED>(p, s0 + lane) : first;
-        int64_t upto = u;
+        const LaneSeq mine = s0 ? lane_seq<PAGED, KT>(p, s0 + lane) : first;
+        int64_t upto = mine.units;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
@@ -148,17 +157,21 @@ __device__ __forceinline__ Place find_unit(const Params &p, int64_t at, int64_t 
             const int l = __ffs(in) - 1;
             Place w;
             w.seq = s0 + l;
-            at -= __shfl_sync(0xffffffffu, upto - u, l);
-            const int64_t head = divide(__shfl_sync(0xffffffffu, u, l), p.a.kv_heads);
+            at -= __shfl_sync(0xffffffffu, upto - mine.units, l);
+            const int64_t head = divide(__shfl_sync(0xffffffffu, mine.units, l), p.a.kv_heads);
             w.kvh = (int)divide(at, head);
             at -= w.kvh * head;
+            q.q0 = __shfl_sync(0xffffffffu, mine.q.q0, l);
+            q.k0 = __shfl_sync(0xffffffffu, mine.q.k0, l);
+            q.nk = __shfl_sync(0xffffffffu, mine.q.nk, l);
+            q.nq = __shfl_sync(0xffffffffu, mine.q.nq, l);
+            q.ok = true;
             // the last row tile that starts at or before `at`: 32 places at a time
-            const ServeSeq q = serve_seq(p.a, w.seq);
             int lo = 0, n = row_tiles<PAGED>(p, q);
             int64_t before = 0;
             while (n > 1) {
                 const int step = (n + 31) / 32, r = lo + lane * step;
-                const int64_t x = lane * step < n ? units_before<PAGED>(p, q, r) : INT64_MAX;
+                const int64_t x = lane * step < n ? units_before<PAGED, KT>(p, q, r) : INT64_MAX;
                 const int k = __popc(__ballot_sync(0xffffffffu, x <= at)) - 1;
                 before = __shfl_sync(0xffffffffu, x, k);
                 lo += k * step;
@@ -183,7 +196,7 @@ struct Segment {
     __device__ __forceinline__ int ctx() const { return nk - nq; }   // keys in front of the sequence's first query
 };
 constexpr int SEG_RING = 4;
-template <bool PAGED>
+template <bool PAGED, int KT>
 struct Walk {
     Place at;
     int64_t left;
@@ -204,7 +217,7 @@ struct Walk {
                 }
                 continue;
             }
-            const int n = key_tiles<PAGED>(p, sq, at.r);
+            const int n = key_tiles<PAGED, KT>(p, sq, at.r);
             const int64_t take = min(left, n + OVERHEAD - at.off), off = at.off;
             g.seq = at.seq;
             g.kvh = at.kvh;
@@ -217,7 +230,7 @@ struct Walk {
             g.t0 = (int)min(off, (int64_t)n);
             g.t1 = (int)min(off + take, (int64_t)n);
             // keys that every row of the unit sees: the context, or what its first token sees
-            g.special = (PAGED ? g.ctx() : max(0, g.token0 + g.ctx() + 1)) / T;
+            g.special = (PAGED ? g.ctx() : max(0, g.token0 + g.ctx() + 1)) / KT;
             left -= take;
             at.off += take;
             if (at.off == n + OVERHEAD) {
@@ -292,6 +305,11 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -341,11 +359,11 @@ __device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *map, int x,
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(tc::su32(bar))
                  : "memory");
 }
-// MN-major, 128-byte swizzle: rows of 64 elements, eight of them to a group of 1 KB; the second 64 columns lie HALF_BYTES further on
+// MN-major, 128-byte swizzle: rows of 64 elements, eight of them to a group of 1 KB; the second 64 columns lie HALF bytes further on
+template <int HALF>
 __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(HALF_BYTES >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(HALF >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-
 // A row's pieces of 16 bytes (32 columns: four of them) turned around among four lanes: piece i is then row (lane & ~3) + i's, its part lane & 3,
 // so that four lanes write 64 bytes of a row side by side instead of 32 lanes to 32 rows
 __device__ __forceinline__ void turn4(uint4 (&w)[4]) {
@@ -382,7 +400,7 @@ __device__ __noinline__ float slow_score(const ServeAttn &a, const ServeSeq &sq,
     return s;
 }
 // part: null where the segment is a whole row tile, else where its (m, l) and sums go (rows of them)
-template <typename E, bool PAGED, int HSP>
+template <typename E, bool PAGED, int KT>
 __device__ __noinline__ void slow_row(const Params &p, const Segment &g, RowView v, int token, int head, float *part, int rows, int prow) {
     ServeSeq sq;
     sq.q0 = g.q0;
@@ -392,7 +410,7 @@ __device__ __noinline__ void slow_row(const Params &p, const Segment &g, RowView
     sq.ok = true;
     const char *q = (const char *)p.a.q + (int64_t)(g.q0 + token) * p.a.q_stride + (int64_t)head * p.a.hs * 2;
     char *dst = (char *)p.a.out + (int64_t)(g.q0 + token) * p.a.out_stride + (int64_t)head * p.a.hs * 2;
-    const int ctx = g.ctx(), k0 = g.t0 * T, k1 = min((int64_t)g.nk, (int64_t)g.t1 * T);
+    const int ctx = g.ctx(), k0 = g.t0 * KT, k1 = min((int64_t)g.nk, (int64_t)g.t1 * KT);
     float m = -CUDART_INF_F, l = 0.f;
     for (int key = k0; key < k1; key++)
         if (sees<PAGED>(v, ctx, key)) m = fmaxf(m, slow_score<E, PAGED>(p.a, sq, g.seq, g.kvh, q, key) * p.scale_log2);
@@ -437,11 +455,12 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     using namespace tc;
     using namespace sat;
     using E = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-    constexpr int NS = stages(HSP, SHARE), TILE = tile_bytes(HSP), HALVES = HSP / 64, NQ = SHARE ? 2 : 1;
+    constexpr int KT = key_tile(SHARE), NS = stages(HSP, SHARE), HALVES = HSP / 64, NQ = SHARE ? 2 : 1;
+    constexpr int QTILE = T * HSP * 2, QHALF = T * 128, TILE = KT * HSP * 2, KHALF = KT * 128;   // bytes; halves: 64 columns
     constexpr uint32_t FMT = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(T >> 4) << 24);
-    constexpr uint32_t IDESC_QK = FMT | ((uint32_t)(T >> 3) << 17), IDESC_PV = FMT | (1u << 16) | ((uint32_t)(HSP >> 3) << 17);
+    constexpr uint32_t IDESC_QK = FMT | ((uint32_t)(KT >> 3) << 17), IDESC_PV = FMT | (1u << 16) | ((uint32_t)(HSP >> 3) << 17);
     extern __shared__ __align__(1024) uint8_t smem[];   // behind 3 KB of the arrays below, so that three stages fill the 227 KB to the byte
-    uint8_t *qs = smem, *ks = qs + NQ * TILE, *vs = ks + NS * TILE;
+    uint8_t *qs = smem, *ks = qs + NQ * QTILE, *vs = ks + NS * TILE;
     __shared__ uint64_t bar_q, bar_qfree, bar_k[NS], bar_kfree[NS], bar_v[NS], bar_vfree[NS], bar_fix[NS], bar_s[2], bar_p[2], bar_o[2], bar_od;
     __shared__ uint32_t tmem_base_s;
     __shared__ int s_fail;
@@ -499,64 +518,77 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         return g.t0 >= 0 && !*fail;
     };
 
-    // The tiles of a segment on their way to a ring of stages (warp 0: keys, warp 3: values), in front of each `before(tile)`
-    auto copy_tiles = [&](uint8_t *ring, const CUtensorMap *map, uint64_t *full, uint64_t *free, int &tile, auto &&before) {
-        // paged: a box per page and 64 columns. The page's row in the pool is looked up a tile ahead, by a lane each; pages that are not needed
-        // and bad ids lie past the pool: zeros. One lane issues (a warp's lanes one after another took 72 cycles per box).
-        const int rows = min(p.a.block_size, T), boxes = T / rows;   // 1 to 16 pages
-        auto page_row = [&](int j) {
-            const int key = j * T + lane * rows;
-            if (lane >= boxes || key >= g.nk || j >= g.t1) return p.pool_rows;
-            const int32_t blk = p.a.tables[(int64_t)g.seq * p.a.max_blocks + key / p.a.block_size];
-            if (blk >= 0 && blk < p.a.pool_blocks) return (blk * p.a.kv_heads + g.kvh) * p.a.block_size + key % p.a.block_size;
-            if (p.a.err) report_error(p.a.err, TLB_ERR_INDEX);
-            return p.pool_rows;
+    // The tiles of a segment on their way to a ring of stages (warp 0: keys, warp 3: values)
+    auto copy_tiles = [&](uint8_t *ring, const CUtensorMap *map, uint64_t *full, uint64_t *free, int &tile, auto &&before, auto &&behind) {
+        // paged: a box per page and 64 columns, a lane each. The page ids are loaded a tile ahead; pages that are not needed and bad ids lie past the
+        // pool: zeros
+        const int bs = p.a.block_size, shift = 31 - __clz(bs), rows = min(bs, KT), pages = KT / rows;   // 1 to 16 of a tile
+        const int pg = lane % pages, h = lane / pages;
+        auto page_id = [&](int j) {
+            const int key = j * KT + pg * rows;
+            return PAGED && h < HALVES && j < g.t1 && key < g.nk ? p.a.tables[(int64_t)g.seq * p.a.max_blocks + (key >> shift)] : -1;
         };
-        int row = PAGED ? page_row(g.t0) : 0;
+        int id = page_id(g.t0);
         for (int j = g.t0; j < g.t1; j++, tile++) {
             before(j);
-            const int ahead = PAGED ? page_row(j + 1) : 0, s = tile % NS;
+            const int s = tile % NS;
+            int row = p.pool_rows;
+            if (PAGED) {
+                const int key = j * KT + pg * rows;
+                if (id >= 0 && id < p.a.pool_blocks) row = (id * p.a.kv_heads + g.kvh) * bs + (key & (bs - 1));
+                else if (h < HALVES && key < g.nk && p.a.err) report_error(p.a.err, TLB_ERR_INDEX);
+                id = page_id(j + 1);
+            }
             mbar_wait_nap(&free[s], (uint32_t)(tile / NS + 1) & 1u, fail, 32);
             if (__any_sync(0xffffffffu, *fail)) return;
             if (lane == 0) mbar_expect_tx(&full[s], TILE);
-            if (!PAGED) {
-                if (lane == 0)
-                    for (int h = 0; h < HALVES; h++) tma_3d(ring + s * TILE + h * HALF_BYTES, map, h * 64, g.kvh, g.k0 + j * T, &full[s]);
-            } else {
-#pragma unroll 4
-                for (int b = 0; b < boxes; b++) {
-                    const int r = __shfl_sync(0xffffffffu, row, b);
-                    if (lane == 0)
-                        for (int h = 0; h < HALVES; h++) tma_2d(ring + s * TILE + h * HALF_BYTES + b * rows * 128, map, h * 64, r, &full[s]);
-                }
+            __syncwarp();
+            if (PAGED) {
+                if (h < HALVES) tma_2d(ring + s * TILE + h * KHALF + pg * rows * 128, map, h * 64, row, &full[s]);
+            } else if (lane < HALVES) {
+                tma_3d(ring + s * TILE + lane * KHALF, map, lane * 64, g.kvh, g.k0 + j * KT, &full[s]);
             }
-            row = ahead;
+            behind(j);
         }
     };
     if (warp == 0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
         // ---- copies. The keys of a segment's first tiles are on their way before its queries, whose room the segment in front still uses.
-        Walk<PAGED> walk;
+        Walk<PAGED, KT> walk;
         {
-            int64_t seq0;
-            const int64_t total = total_units<PAGED>(p, seq0), share = share_of(p, total), first = share * blockIdx.x;
+            LaneSeq seq0;
+            const int64_t total = total_units<PAGED, KT>(p, seq0), share = share_of(p, total), first = share * blockIdx.x;
             if (lane == 0 && blockIdx.x == 0) p.ends[p.ctas].off = share;
             walk.left = min(share, total - first);
-            walk.at = walk.left > 0 ? find_unit<PAGED>(p, first, seq0) : Place{p.a.seqs, 0, 0, 0};
+            walk.at = {p.a.seqs, 0, 0, 0};
+            if (walk.left > 0) {
+                walk.at = find_unit<PAGED, KT>(p, first, seq0, walk.sq);
+                walk.tiles = row_tiles<PAGED>(p, walk.sq);
+                walk.loaded = walk.at.seq;
+            }
         }
-        auto tell = [&]() {
+        auto tell = [&](const Segment &x) {
             const int r = g_at % SEG_RING;
             mbar_wait_nap(&bar_segfree[r], (uint32_t)(g_at / SEG_RING + 1) & 1u, fail, 32);
             if (lane == 0) {
-                segs[r] = g;
+                segs[r] = x;
                 mbar_arrive(&bar_seg[r]);
             }
             g_at++;
         };
         int tile = 0, seg = 0;
-        while (walk.next(p, g)) {
-            tell();
-            if (g.t1 == g.t0) continue;   // a row tile that sees nothing has no part in the pipeline's counts
+        Segment ahead;
+        auto look_ahead = [&]() {
+            if (!walk.next(p, ahead)) ahead.t0 = -1;
+            tell(ahead);
+        };
+        look_ahead();
+        while (ahead.t0 >= 0 && !__any_sync(0xffffffffu, *fail)) {
+            g = ahead;
+            if (g.t1 == g.t0) {   // a row tile that sees nothing has no part in the pipeline's counts
+                look_ahead();
+                continue;
+            }
             bool have_q = false;
             auto load_q = [&]() {
                 if (lane == 0) {
@@ -564,20 +596,21 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                     mbar_expect_tx(&bar_q, (uint32_t)(NQ * HALVES * 128 * p.group * p.tpt));
                     for (int x = 0; x < NQ; x++)
                         for (int h = 0; h < HALVES; h++)
-                            tma_3d(qs + x * TILE + h * HALF_BYTES, &p.q, h * 64, g.kvh * p.group, g.q0 + g.token0 + x * p.tpt, &bar_q);
+                            tma_3d(qs + x * QTILE + h * QHALF, &p.q, h * 64, g.kvh * p.group, g.q0 + g.token0 + x * p.tpt, &bar_q);
                 }
                 have_q = true;
             };
+            const int look_at = min(g.t0 + 1, g.t1 - 1);
             copy_tiles(ks, &p.k, bar_k, bar_kfree, tile, [&](int j) {
                 if (!have_q && (j - g.t0 >= NS || __any_sync(0xffffffffu, mbar_test(su32(&bar_qfree), (uint32_t)(seg + 1) & 1u)))) load_q();
+            }, [&](int j) {
+                if (j == look_at) look_ahead();   // the next segment, while this one's tiles are on their way
             });
             if (__any_sync(0xffffffffu, *fail)) break;
             if (!have_q) load_q();
             __syncwarp();
             seg++;
         }
-        g.t0 = -1;
-        tell();
         if (lane == 0) p.ends[blockIdx.x] = walk.left == 0 ? walk.at : Place{p.a.seqs, 0, 0, 0};
     } else if (warp == 1) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
@@ -590,12 +623,11 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             if (n == 0) continue;
             auto issue_s = [&](int i) {
                 const int x = i & 1, k = tile + (SHARE ? i >> 1 : i), s = k % NS;
-                if (!SHARE || x == 0) mbar_wait_nap(&bar_k[s], (uint32_t)(k / NS) & 1u, fail, 0);
                 tc_fence_after();
                 if (leader) {
 #pragma unroll
                     for (int h = 0; h < HALVES; h++) {
-                        const uint64_t qd = plain::desc_sw128(su32(qs + (SHARE ? x * TILE : 0) + h * HALF_BYTES)), kd = plain::desc_sw128(su32(ks + s * TILE + h * HALF_BYTES));
+                        const uint64_t qd = plain::desc_sw128(su32(qs + (SHARE ? x * QTILE : 0) + h * QHALF)), kd = plain::desc_sw128(su32(ks + s * TILE + h * KHALF));
 #pragma unroll
                         for (int e = 0; e < 4; e++) umma_f16(tmem + (uint32_t)(x * T), qd + 2 * e, kd + 2 * e, IDESC_QK, (h | e) ? 1u : 0u);
                     }
@@ -605,25 +637,53 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 }
                 __syncwarp();
             };
-            mbar_wait_nap(&bar_q, (uint32_t)seg & 1u, fail, 0);
-            issue_s(0);
-            if (steps > 1) issue_s(1);
-            for (int i = 0; i < steps; i++) {
-                const int x = i & 1, j = SHARE ? i >> 1 : i, k = tile + j, s = k % NS;
-                if (!SHARE || x == 0) mbar_wait_nap(&bar_fix[s], (uint32_t)(k / NS) & 1u, fail, 0);
-                mbar_wait_nap(&bar_p[x], (n_p[x]++) & 1u, fail, 0);
+            auto issue_o = [&](int i) {
+                const int x = i & 1, s = (tile + (SHARE ? i >> 1 : i)) % NS;
                 if (i == 0 && seg > 0) mbar_wait_nap(&bar_od, (uint32_t)(seg - 1) & 1u, fail, 0);
                 tc_fence_after();
                 if (leader) {
-                    const uint64_t vd = desc_mn(su32(vs + s * TILE));
+                    const uint64_t vd = desc_mn<KHALF>(su32(vs + s * TILE));
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
+                    for (int e = 0; e < KT / 16; e++)
                         umma_f16_ta(tmem + O_COL + (uint32_t)(x * T), tmem + (uint32_t)(x * T + e * 8), vd + (uint64_t)(e * 128), IDESC_PV, (i > 1 || e) ? 1u : 0u);
                     umma_commit(&bar_o[x]);
                     if (!SHARE || x == 1) umma_commit(&bar_vfree[s]);
                 }
                 __syncwarp();
-                if (i + 2 < steps) issue_s(i + 2);
+                n_p[x]++;
+            };
+            auto k_bar = [&](int i) { return &bar_k[(tile + (SHARE ? i >> 1 : i)) % NS]; };
+            auto v_bar = [&](int i) { return &bar_fix[(tile + (SHARE ? i >> 1 : i)) % NS]; };
+            auto parity = [&](int i) { return (uint32_t)((tile + (SHARE ? i >> 1 : i)) / NS) & 1u; };
+            mbar_wait_nap(&bar_q, (uint32_t)seg & 1u, fail, 0);
+            if (SHARE) {
+                mbar_wait_nap(k_bar(0), parity(0), fail, 0);
+                issue_s(0);
+                issue_s(1);
+                for (int i = 0; i < steps; i++) {
+                    if ((i & 1) == 0) mbar_wait_nap(v_bar(i), parity(i), fail, 0);
+                    mbar_wait_nap(&bar_p[i & 1], n_p[i & 1] & 1u, fail, 0);
+                    issue_o(i);
+                    if (i + 2 < steps) {
+                        if ((i & 1) == 0) mbar_wait_nap(k_bar(i + 2), parity(i + 2), fail, 0);
+                        issue_s(i + 2);
+                    }
+                }
+            } else {
+                // (taking a P that is ready before keys that are not, so that a tile of values is free sooner: 185 us against 177 at 48 x 4096)
+                for (int i = 0; i < min(2, steps); i++) {
+                    mbar_wait_nap(k_bar(i), parity(i), fail, 0);
+                    issue_s(i);
+                }
+                for (int i = 0; i < steps; i++) {
+                    mbar_wait_nap(v_bar(i), parity(i), fail, 0);
+                    mbar_wait_nap(&bar_p[i & 1], n_p[i & 1] & 1u, fail, 0);
+                    issue_o(i);
+                    if (i + 2 < steps) {
+                        mbar_wait_nap(k_bar(i + 2), parity(i + 2), fail, 0);
+                        issue_s(i + 2);
+                    }
+                }
             }
             tile += n;
             seg++;
@@ -639,22 +699,22 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 const int s = tile % NS;
                 mbar_wait_nap(&bar_v[s], (uint32_t)(tile / NS) & 1u, fail, 0);
                 if (j >= g.special) {
-                    const int live = min(T, g.nk - j * T);
+                    const int live = min(KT, g.nk - j * KT);
                     uint4 *v = reinterpret_cast<uint4 *>(vs + s * TILE);
-                    constexpr uint32_t EXP = BF16 ? 0x7f807f80u : 0x7c007c00u;
+                    constexpr uint32_t EXP = BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = BF16 ? 0x00800080u : 0x04000400u;   // one more than all ones carries into the sign
                     uint32_t odd = 0;
 #pragma unroll 8
                     for (int i = lane; i < TILE / 16; i += 32) {
-                        if (((i >> 3) & (T - 1)) >= live) {
+                        if (((i >> 3) & (KT - 1)) >= live) {
                             v[i] = make_uint4(0, 0, 0, 0);
                         } else {
                             const uint4 w = v[i];
-                            odd |= __vcmpeq2(w.x & EXP, EXP) | __vcmpeq2(w.y & EXP, EXP) | __vcmpeq2(w.z & EXP, EXP) | __vcmpeq2(w.w & EXP, EXP);
+                            odd |= ((w.x & EXP) + ONE) | ((w.y & EXP) + ONE) | ((w.z & EXP) + ONE) | ((w.w & EXP) + ONE);
                         }
                     }
-                    if (odd) slow_ring[seg % SLOW_RING] = seg + 1;
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    if (odd & 0x80008000u) slow_ring[seg % SLOW_RING] = seg + 1;
                 }
+                if (j >= g.special) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_fix[s]);
             }
@@ -663,7 +723,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     } else if (warp == 3) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
         int tile = 0;
-        while (next()) copy_tiles(vs, &p.v, bar_v, bar_vfree, tile, [](int) {});
+        while (next()) copy_tiles(vs, &p.v, bar_v, bar_vfree, tile, [](int) {}, [](int) {});
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_STREAMS));
         // ---- the streams
@@ -690,9 +750,9 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 const int j = g.t0 + (SHARE ? i : 2 * i + x);
                 mbar_wait_nap(&bar_s[x], (done[x] + i) & 1u, fail, 0);
                 tc_fence_after();
-                float y[T];
+                float y[KT];
 #pragma unroll
-                for (int c = 0; c < 4; c++) ld32(s_at + 32 * c, y + 32 * c);
+                for (int c = 0; c < KT / 32; c++) ld32(s_at + 32 * c, y + 32 * c);
                 tmem_ld_wait();
                 if (j >= g.special) {
                     if (PAGED && !have_bits) {
@@ -700,8 +760,8 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                         have_bits = true;
                     }
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const uint32_t seen = seen32<PAGED>(view, ctx, j * T + 32 * c);
+                    for (int c = 0; c < KT / 32; c++) {
+                        const uint32_t seen = seen32<PAGED>(view, ctx, j * KT + 32 * c);
 #pragma unroll
                         for (int e = 0; e < 32; e++)
                             if (!((seen >> e) & 1u)) y[32 * c + e] = -CUDART_INF_F;
@@ -709,10 +769,12 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 }
                 float mxs[4] = {y[0], y[1], y[2], y[3]};   // four chains
 #pragma unroll
-                for (int e = 4; e < T; e += 4)
+                for (int e = 4; e + 8 <= KT; e += 8)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) mxs[c] = fmaxf(mxs[c], y[e + c]);
-                const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * p.scale_log2;
+                    for (int c = 0; c < 4; c++) mxs[c] = max3(mxs[c], y[e + c], y[e + 4 + c]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) mxs[c] = fmaxf(mxs[c], y[KT - 4 + c]);
+                const float mx = fmaxf(max3(mxs[0], mxs[1], mxs[2]), mxs[3]) * p.scale_log2;
                 float alpha = 1.f;
                 if (!have_ref) {
                     if (mx != -CUDART_INF_F) {
@@ -740,7 +802,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 const uint64_t sc = pack2(p.scale_log2, p.scale_log2), ref = pack2(-m_ref, -m_ref);
                 uint64_t sums[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
+                for (int c = 0; c < KT / 64; c++) {
                     uint32_t w[32];
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
@@ -771,7 +833,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             const int prow = (SHARE ? x * T : 0) + row;
             if (slow) {
                 if (PAGED && !have_bits) view.bits = ancestors_of(parents, token & 63, p.a.err);
-                if (live_row && (SHARE || x == 0)) slow_row<E, PAGED, HSP>(p, g, view, token, head, part, NQ * T, prow);
+                if (live_row && (SHARE || x == 0)) slow_row<E, PAGED, KT>(p, g, view, token, head, part, NQ * T, prow);
                 __syncwarp();
             } else {
                 float f_mine = 1.f, f_other = 0.f;
@@ -875,7 +937,7 @@ __global__ void __launch_bounds__(128) k_serve_join(const __grid_constant__ sat:
     const Place v = c ? p.ends[c - 1] : Place{0, 0, 0, 0};
     if (v.off > 0 && v.seq == w.seq && v.kvh == w.kvh && v.r == w.r) return;   // it begins in a stretch in front
     const ServeSeq sq = serve_seq(p.a, w.seq);
-    const int n = key_tiles<PAGED>(p, sq, w.r);
+    const int n = key_tiles<PAGED, key_tile(SHARE)>(p, sq, w.r);
     if (w.off >= n) return;   // all of its key tiles lie in this stretch
     const int parts = 1 + (int)((n - w.off + p.ends[p.ctas].off - 1) / p.ends[p.ctas].off);
     // 32 rows: a lane's row is its own, a warp's columns a quarter of them
@@ -884,25 +946,28 @@ __global__ void __launch_bounds__(128) k_serve_join(const __grid_constant__ sat:
     if (rr >= p.tpt * p.group || token >= (PAGED ? p.a.drafts : sq.nq)) return;
     auto slot = [&](int i) { return p.partial + ((size_t)(c + i) * 2 + (i ? 0 : 1)) * SLOT; };
     float m = -CUDART_INF_F;
+#pragma unroll 4
     for (int i = 0; i < parts; i++) {
         const float2 ml = *reinterpret_cast<const float2 *>(slot(i) + row * 2);
-        if (ml.y != 0.f) m = fmaxf(m, ml.x);   // else the row sees nothing in this part
+        m = fmaxf(m, ml.y == 0.f ? -CUDART_INF_F : ml.x);   // l = 0: the row sees nothing in this part
     }
     if (m == -CUDART_INF_F) m = 0.f;
     float l = 0.f;
     float4 o[HSP / 16];
 #pragma unroll
     for (int e = 0; e < HSP / 16; e++) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
     for (int i = 0; i < parts; i++) {
         const float2 ml = *reinterpret_cast<const float2 *>(slot(i) + row * 2);
-        if (ml.y == 0.f) continue;
-        const float f = ex2(ml.x - m);
-        l = fmaf(ml.y, f, l);
         const float4 *s = reinterpret_cast<const float4 *>(slot(i) + ROWS * 2) + (size_t)(warp * (HSP / 16)) * ROWS + row;
+        float4 y[HSP / 16];
 #pragma unroll
-        for (int e = 0; e < HSP / 16; e++) {
-            const float4 y = s[(size_t)e * ROWS];
-            o[e] = make_float4(fmaf(y.x, f, o[e].x), fmaf(y.y, f, o[e].y), fmaf(y.z, f, o[e].z), fmaf(y.w, f, o[e].w));
+        for (int e = 0; e < HSP / 16; e++) y[e] = s[(size_t)e * ROWS];
+        if (ml.y != 0.f) {
+            const float f = ex2(ml.x - m);
+            l = fmaf(ml.y, f, l);
+#pragma unroll
+            for (int e = 0; e < HSP / 16; e++) o[e] = make_float4(fmaf(y[e].x, f, o[e].x), fmaf(y[e].y, f, o[e].y), fmaf(y[e].z, f, o[e].z), fmaf(y[e].w, f, o[e].w));
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -930,7 +995,7 @@ static int sat_ctas(const ServeAttn &a, int sm_count) {
     const bool share = sat_share(a);
     const int64_t tt = (int64_t)(sat::T / (a.heads / a.kv_heads)) * (share ? 2 : 1);
     const int64_t tiles = a.paged ? (a.drafts + tt - 1) / tt * a.seqs : a.q_rows / tt + a.seqs;
-    const int64_t keys = a.paged ? ((int64_t)a.max_blocks * a.block_size + sat::T - 1) / sat::T : (a.kv_rows + sat::T - 1) / sat::T;
+    const int64_t kt = sat::key_tile(share), keys = a.paged ? ((int64_t)a.max_blocks * a.block_size + kt - 1) / kt : (a.kv_rows + kt - 1) / kt;
     const double units = (double)tiles * a.kv_heads * (double)(keys + sat::OVERHEAD);
     return units / 2 < sm_count ? std::max(1, (int)(units / 2 + 1)) : sm_count;
 }
@@ -973,7 +1038,10 @@ cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count
     p.tpt = T / p.group;
     const bool share = sat_share(a);
     p.tt = p.tpt * (share ? 2 : 1);
-    p.min_units = 1 + OVERHEAD;
+#ifndef MINU
+#define MINU 3
+#endif
+    p.min_units = MINU;
     const uint64_t hs = (uint64_t)a.hs;
     cudaError_t e;
     {
@@ -981,17 +1049,18 @@ cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count
         const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)p.tpt};
         e = tc_encode_sw128(&p.q, a.q, 3, dims, strides, box, a.bf16);
     }
+    const uint32_t kt = (uint32_t)key_tile(share);
     for (int i = 0; i < 2 && e == cudaSuccess; i++) {
         if (a.paged) {
             p.pool_rows = (int)(a.pool_blocks * a.kv_heads * a.block_size);
             const uint64_t dims[2] = {hs, (uint64_t)p.pool_rows}, strides[1] = {hs * 2};
-            const uint32_t box[2] = {64, (uint32_t)std::min(a.block_size, T)};
+            const uint32_t box[2] = {64, std::min((uint32_t)a.block_size, kt)};
             e = tc_encode_sw128(i ? &p.v : &p.k, i ? a.v : a.k, 2, dims, strides, box, false);
-        } else {
-            const uint64_t dims[3] = {hs, (uint64_t)a.kv_heads, (uint64_t)a.kv_rows}, strides[2] = {hs * 2, (uint64_t)(i ? a.v_stride : a.k_stride)};
-            const uint32_t box[3] = {64, 1, T};
-            e = tc_encode_sw128(i ? &p.v : &p.k, i ? a.v : a.k, 3, dims, strides, box, a.bf16);
+            continue;
         }
+        const uint64_t dims[3] = {hs, (uint64_t)a.kv_heads, (uint64_t)a.kv_rows}, strides[2] = {hs * 2, (uint64_t)(i ? a.v_stride : a.k_stride)};
+        const uint32_t box[3] = {64, 1, kt};
+        e = tc_encode_sw128(i ? &p.v : &p.k, i ? a.v : a.k, 3, dims, strides, box, a.bf16);
     }
     if (e != cudaSuccess) return e;
     const int ctas = p.ctas = sat_ctas(a, sm_count);
