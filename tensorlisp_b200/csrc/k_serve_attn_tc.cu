@@ -46,10 +46,12 @@ constexpr float RESCALE_STEP = 8.f;     // in the base-2 domain
 constexpr uint32_t O_COL = 256;         // S / P of stream x at column 128 x, O at 256 + 128 x
 constexpr int SLOW_RING = 16;
 constexpr int REGS_ROLES = 88, REGS_STREAMS = 200;   // registers of a thread (setmaxnreg): the streams hold a row of 128 scores
-constexpr int OVERHEAD = 2;             // what a row tile costs beside its key tiles, in key tiles
 
 // Keys of a tile. 64 without SHARE: a tile of values is held for a shorter time and more of them are on their way in the same room
 __host__ __device__ constexpr int key_tile(bool share) { return share ? 128 : 64; }
+// What a row tile costs beside its key tiles, in key tiles, and with it a CTA's least share. us with 1, 2, 4, 6: 1 x 8192 546, 506, 500, 511; tree 48 x 32 over
+// up to 8192 182, 180, 174, 172
+__host__ __device__ constexpr int overhead(int kt) { return kt == 128 ? 3 : 5; }
 __host__ __device__ constexpr int stages(int hsp, bool share) { return hsp == 128 ? (share ? 2 : 6) : (share ? 4 : 8); }
 __host__ __device__ constexpr int smem_bytes(int hsp, bool share) { return ((share ? 2 : 1) * T + 2 * stages(hsp, share) * key_tile(share)) * hsp * 2; }
 
@@ -99,7 +101,7 @@ __device__ __forceinline__ int key_tiles(const Params &p, const ServeSeq &s, int
 // units of row tiles [0, r)
 template <bool PAGED, int KT>
 __device__ __forceinline__ int64_t units_before(const Params &p, const ServeSeq &s, int r) {
-    int64_t u = (int64_t)r * OVERHEAD;
+    int64_t u = (int64_t)r * overhead(KT);
     if (PAGED) return u + (int64_t)min(r, (s.nq + p.tt - 1) / p.tt) * ((s.nk + KT - 1) / KT);
     const int R = row_tiles<false>(p, s);
     const int full = min(r, R - 1);
@@ -218,7 +220,7 @@ struct Walk {
                 continue;
             }
             const int n = key_tiles<PAGED, KT>(p, sq, at.r);
-            const int64_t take = min(left, n + OVERHEAD - at.off), off = at.off;
+            const int64_t take = min(left, n + overhead(KT) - at.off), off = at.off;
             g.seq = at.seq;
             g.kvh = at.kvh;
             g.token0 = at.r * p.tt;
@@ -233,7 +235,7 @@ struct Walk {
             g.special = (PAGED ? g.ctx() : max(0, g.token0 + g.ctx() + 1)) / KT;
             left -= take;
             at.off += take;
-            if (at.off == n + OVERHEAD) {
+            if (at.off == n + overhead(KT)) {
                 at.off = 0;
                 at.r++;
             }
@@ -996,8 +998,8 @@ static int sat_ctas(const ServeAttn &a, int sm_count) {
     const int64_t tt = (int64_t)(sat::T / (a.heads / a.kv_heads)) * (share ? 2 : 1);
     const int64_t tiles = a.paged ? (a.drafts + tt - 1) / tt * a.seqs : a.q_rows / tt + a.seqs;
     const int64_t kt = sat::key_tile(share), keys = a.paged ? ((int64_t)a.max_blocks * a.block_size + kt - 1) / kt : (a.kv_rows + kt - 1) / kt;
-    const double units = (double)tiles * a.kv_heads * (double)(keys + sat::OVERHEAD);
-    return units / 2 < sm_count ? std::max(1, (int)(units / 2 + 1)) : sm_count;
+    const double units = (double)tiles * a.kv_heads * (double)(keys + sat::overhead((int)kt)), least = 1 + sat::overhead((int)kt);
+    return units / least < sm_count ? std::max(1, (int)(units / least + 1)) : sm_count;
 }
 static uint64_t sat_ends_bytes(int ctas) { return ((uint64_t)(ctas + 1) * sizeof(sat::Place) + 255) / 256 * 256; }   // the last one: the size of a share
 uint64_t serve_attn_tc_scratch_bytes(const ServeAttn &a, int sm_count) {
@@ -1038,10 +1040,7 @@ cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count
     p.tpt = T / p.group;
     const bool share = sat_share(a);
     p.tt = p.tpt * (share ? 2 : 1);
-#ifndef MINU
-#define MINU 3
-#endif
-    p.min_units = MINU;
+    p.min_units = 1 + overhead(key_tile(share));
     const uint64_t hs = (uint64_t)a.hs;
     cudaError_t e;
     {
