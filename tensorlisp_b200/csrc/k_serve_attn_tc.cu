@@ -877,14 +877,24 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                     float o[32];
                     ld32(o_at + c0, o);
                     tmem_ld_wait();
+                    // a stream without a tile has left nothing there; a row that sees nothing has sums of zero, but a row of padding may hold anything
+                    if (mine > 0) {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = mine > 0 && view.lim >= 0 ? o[e] * f_mine : 0.f;
-                    if (!SHARE) {
+                        for (int e = 0; e < 32; e++) o[e] *= f_mine;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = 0.f;
+                    }
+                    if (!SHARE && other > 0) {
                         float o2[32];
                         ld32(lanes + O_COL + (uint32_t)((x ^ 1) * T) + c0, o2);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = other > 0 && view.lim >= 0 ? fmaf(o2[e], f_other, o[e]) : o[e];
+                        for (int e = 0; e < 32; e++) o[e] = fmaf(o2[e], f_other, o[e]);
+                    }
+                    if (PAGED && view.lim < 0) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = 0.f;
                     }
                     if (whole) {
                         uint4 w[4];
@@ -993,11 +1003,12 @@ bool serve_attn_tc_supported(const ServeAttn &a) {
 }
 // A pair of row tiles per unit where sequences fill them on average.
 static bool sat_share(const ServeAttn &a) { return !a.paged && a.q_rows * (a.heads / a.kv_heads) > (int64_t)a.seqs * sat::T; }
+static int64_t most_key_tiles(const ServeAttn &a, int kt) { return ((a.paged ? (int64_t)a.max_blocks * a.block_size : a.kv_rows) + kt - 1) / kt; }
 static int sat_ctas(const ServeAttn &a, int sm_count) {
     const bool share = sat_share(a);
     const int64_t tt = (int64_t)(sat::T / (a.heads / a.kv_heads)) * (share ? 2 : 1);
     const int64_t tiles = a.paged ? (a.drafts + tt - 1) / tt * a.seqs : a.q_rows / tt + a.seqs;
-    const int64_t kt = sat::key_tile(share), keys = a.paged ? ((int64_t)a.max_blocks * a.block_size + kt - 1) / kt : (a.kv_rows + kt - 1) / kt;
+    const int64_t kt = sat::key_tile(share), keys = most_key_tiles(a, (int)kt);
     const double units = (double)tiles * a.kv_heads * (double)(keys + sat::overhead((int)kt)), least = 1 + sat::overhead((int)kt);
     return units / least < sm_count ? std::max(1, (int)(units / least + 1)) : sm_count;
 }
@@ -1009,7 +1020,8 @@ uint64_t serve_attn_tc_scratch_bytes(const ServeAttn &a, int sm_count) {
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
 static cudaError_t sat_launch(const sat::Params &p, int ctas, cudaStream_t st) {
     cudaError_t e = launch_pdl(k_serve_attn_tc<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas), dim3(sat::THREADS), sat::smem_bytes(HSP, SHARE), st, p);
-    if (e == cudaSuccess && ctas > 1) e = launch_pdl(k_serve_join<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas - 1, (SHARE ? 2 : 1) * sat::T / 32), dim3(128), 0, st, p);
+    if (e == cudaSuccess && ctas > 1 && most_key_tiles(p.a, sat::key_tile(SHARE)) > 1)   // a single key tile is never cut
+        e = launch_pdl(k_serve_join<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas - 1, (SHARE ? 2 : 1) * sat::T / 32), dim3(128), 0, st, p);
     return e;
 }
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
