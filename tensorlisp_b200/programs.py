@@ -249,6 +249,77 @@ def prefill_step(cfg: DecoderConfig, n_seqs: int, n_tokens: int, tp: int = 1, wr
     return DecoderGraph(g, specs, [pool_elems * 2] * (2 * len(pools)), names, logits, -1, cfg, tp)
 
 
+def _layer(g: Graph, cfg: DecoderConfig, wid: dict, i: int, x: int, pos: int, slots: int, pools: tuple, T: int, attend) -> int:
+    """One layer for T tokens whose keys and values go to the paged pools; attend(q16, k16, v16) -> the f16 attention result [hd, heads, T]."""
+    p, hd = "blk.%d." % i, cfg.head_dim
+    heads, kvh = cfg.n_heads, cfg.n_kv_heads
+    h = rms_norm_w(g, x, wid[p + "attn_norm"], cfg.eps, p + "attn_in")
+    q = g.mul_mat(wid[p + "wq"], h, p + "q")
+    k = g.mul_mat(wid[p + "wk"], h, p + "k")
+    v = g.mul_mat(wid[p + "wv"], h, p + "v")
+    q = g.set_name(rope_neox(g, g.reshape(q, [hd, heads, T]), pos, hd, cfg.rope_theta), p + "q_rope")
+    k = g.set_name(rope_neox(g, g.reshape(k, [hd, kvh, T]), pos, hd, cfg.rope_theta), p + "k_rope")
+    k16 = g.cast(g.reshape(k, [hd * kvh, T]), F16, p + "k16")
+    v16 = g.cast(v, F16, p + "v16")
+    g.paged_cache_write(k16, v16, pools[0], pools[1], slots, cfg.block_size, kvh, p + "cache_write")
+    a = attend(g.cast(q, F16, p + "q16"), g.reshape(k16, [hd, kvh, T]), g.reshape(v16, [hd, kvh, T]))
+    x = g.add(x, g.mul_mat(wid[p + "wo"], g.reshape(g.cast(a, F32), [hd * heads, T]), p + "attn_out"), p + "res1")
+    f = swiglu_ffn(g, x, wid[p + "ffn_norm"], wid[p + "ffn_gate"], wid[p + "ffn_up"], wid[p + "ffn_down"], cfg.eps, p)
+    return g.add(x, f, p + "res2")
+
+
+def packed_prefill_step(cfg: DecoderConfig, n_seqs: int, n_tokens: int, pool_blocks: int) -> DecoderGraph:
+    """The prompts of `n_seqs` sequences in one pass, packed one behind the other without padding: `n_tokens` rows hold all of them (rows behind the
+    last one are computed and ignored; their cache slots are negative). Inputs: token ids [n_tokens], positions, the offsets [n_seqs + 1] of the
+    prompts, the row index of every prompt's last token, the cache slots. Logits for the last token of every prompt."""
+    g = Graph()
+    specs = decoder_weights(cfg)
+    wid = {s.name: g.weight(s.ty, s.ne, s.name) for s in specs}
+    pool_elems = pool_blocks * cfg.n_kv_heads * cfg.block_size * cfg.head_dim
+    pools = [(g.state(F16, [pool_elems], "k_pool.%d" % i), g.state(F16, [pool_elems], "v_pool.%d" % i)) for i in range(cfg.n_layers)]
+    ids, pos = g.input(I32, [n_tokens], "ids"), g.input(I32, [n_tokens], "pos")
+    offsets, last = g.input(I32, [n_seqs + 1], "offsets"), g.input(I32, [n_seqs], "last")
+    slots = g.input(I32, [2 * n_tokens], "slots")
+    scale = 1.0 / float(np.sqrt(cfg.head_dim))
+    x = g.get_rows(wid["token_embd"], ids, "embd")
+    for i in range(cfg.n_layers):
+        x = _layer(g, cfg, wid, i, x, pos, slots, pools[i], n_tokens,
+                   lambda q, k, v: g.packed_attention(q, k, v, offsets, scale, name="blk.%d.attn" % i))
+    x = rms_norm_w(g, g.get_rows(x, last, "last_rows"), wid["output_norm"], cfg.eps, "final_norm")
+    logits = g.output(g.mul_mat(wid["output"], x, "logits"))
+    return DecoderGraph(g, specs, [pool_elems * 2] * (2 * cfg.n_layers), dict(ids=0, pos=1, offsets=2, last=3, slots=4), logits, -1, cfg)
+
+
+def verify_step(cfg: DecoderConfig, batch: int, drafts: int, max_ctx: int, pool_blocks: int, top: int = 0) -> DecoderGraph:
+    """One pass over `drafts` drafted tokens of every sequence, which form a tree behind the cached context (speculative decoding). Inputs: token
+    ids [batch * drafts] (sequence by sequence), their positions (context + depth in the tree), block tables, context lengths, how many
+    drafts each sequence has, the drafts' parents [batch, drafts] (-1: the context), the cache slots of the drafts (position context + index of
+    the block table; negative for padding), and a token per draft to score. Outputs: the logits of every draft, its argmax, and `scores`
+    (``Graph.token_logprobs`` with `top` alternatives)."""
+    g = Graph()
+    specs = decoder_weights(cfg)
+    wid = {s.name: g.weight(s.ty, s.ne, s.name) for s in specs}
+    T, kvh, hd = batch * drafts, cfg.n_kv_heads, cfg.head_dim
+    max_blocks = (max_ctx + cfg.block_size - 1) // cfg.block_size
+    pool_elems = pool_blocks * kvh * cfg.block_size * hd
+    pools = [(g.state(F16, [pool_elems], "k_pool.%d" % i), g.state(F16, [pool_elems], "v_pool.%d" % i)) for i in range(cfg.n_layers)]
+    ids, pos = g.input(I32, [T], "ids"), g.input(I32, [T], "pos")
+    tables, context = g.input(I32, [max_blocks, batch], "tables"), g.input(I32, [batch], "context")
+    counts, parents = g.input(I32, [batch], "counts"), g.input(I32, [drafts, batch], "parents")
+    slots, targets = g.input(I32, [2 * T], "slots"), g.input(I32, [T], "targets")
+    scale = 1.0 / float(np.sqrt(hd))
+    x = g.get_rows(wid["token_embd"], ids, "embd")
+    for i in range(cfg.n_layers):
+        x = _layer(g, cfg, wid, i, x, pos, slots, pools[i], T, lambda q, k, v: g.paged_tree_attention(
+            g.reshape(q, [hd, cfg.n_heads, drafts, batch]), pools[i][0], pools[i][1], tables, context, counts, parents, cfg.block_size, scale, kvh, "blk.%d.attn" % i))
+    x = rms_norm_w(g, x, wid["output_norm"], cfg.eps, "final_norm")
+    logits = g.output(g.mul_mat(wid["output"], x, "logits"))
+    token = g.output(g.cast(g.argmax(logits, "argmax"), F32, "token"))
+    scores = g.output(g.token_logprobs(logits, targets, top, "scores"))
+    return DecoderGraph(g, specs, [pool_elems * 2] * (2 * cfg.n_layers),
+                        dict(ids=0, pos=1, tables=2, context=3, counts=4, parents=5, slots=6, targets=7), logits, token, cfg, extras=dict(scores=scores))
+
+
 class DecodeLoop:
     """The host side of a batched greedy decode loop over the paged pool: the loop of ports/gemma4/concurrency.ss:120-158
     (the reference's callers in crates/tensorlisp/tests/native_concurrency.rs:100-143 drive it step by step). One compiled
@@ -307,3 +378,110 @@ class DecodeLoop:
 
     def free(self) -> None:
         self.prog.free()
+
+
+class TreeDecodeLoop:
+    """A greedy decode loop that takes several tokens a step where the caller's drafts are right: the drafts of every sequence form a tree behind the
+    token that is due, one pass (``verify_step``) says which token follows each of them, and the longest path that agrees is kept -- its keys and
+    values are moved into place in the cache (``device_ops.cache_keep``), what else the pass wrote there is overwritten by the next one. The tokens are
+    those of ``DecodeLoop``, up to the rounding of two attention kernels. Block tables are assigned up front for `max_ctx` tokens per sequence."""
+
+    def __init__(self, native, cfg: DecoderConfig, batch: int, drafts: int, max_ctx: int, tables: np.ndarray, top: int = 0) -> None:
+        from .native import NativeProgram
+
+        self.native, self.cfg, self.batch, self.drafts, self.max_ctx = native, cfg, batch, drafts, max_ctx
+        self.tables = np.ascontiguousarray(tables, np.int32)
+        max_blocks = (max_ctx + cfg.block_size - 1) // cfg.block_size
+        assert self.tables.shape == (batch, max_blocks)
+        self.pool_blocks = int(self.tables.max()) + 1
+        self.dg = verify_step(cfg, batch, drafts, max_ctx, self.pool_blocks, top)
+        if not native.state_offsets:
+            native.alloc_states(self.dg.state_bytes)
+        self.prog = NativeProgram.compile(native, self.dg.graph)
+        self.prog.set_input(self.dg.inputs["tables"], self.tables)
+        # what cache_keep reads, beside the pools: tables, context, counts, path, status
+        self.room = native._zeroed(4 * (self.tables.size + batch * (2 + drafts) + 1))
+        self.room.write(0, self.tables)
+        self.context = self.due = None
+        self.steps = 0
+
+    def begin(self, first_ids: np.ndarray, cached_tokens: np.ndarray) -> None:
+        """`first_ids`: the token each sequence feeds first; `cached_tokens`: how many tokens of it the pools already hold."""
+        self.due = np.ascontiguousarray(first_ids, np.int32).copy()
+        self.context = np.ascontiguousarray(cached_tokens, np.int32).copy()
+        self.steps = 0
+
+    def step(self, drafted: list) -> list:
+        """`drafted`: per sequence a list of (token, parent) with parent -1 for what may follow the token that is due, else the index of an earlier
+        entry. Returns the tokens that each sequence has gained: the one that was due is now cached, and so are the accepted drafts; the last one of
+        the list is due next."""
+        B, D, bs = self.batch, self.drafts, self.cfg.block_size
+        assert self.due is not None and len(drafted) == B and all(len(d) < D for d in drafted)
+        assert all(int(c) + 1 + len(d) <= self.max_ctx for c, d in zip(self.context, drafted)), "a sequence outgrows its block table"
+        ids, parents, depth = np.zeros((B, D), np.int32), np.full((B, D), -1, np.int32), np.zeros((B, D), np.int32)
+        slots, targets = np.full((B, D), -1, np.int64), np.full((B, D), -1, np.int32)
+        counts = np.array([1 + len(d) for d in drafted], np.int32)
+        for b, d in enumerate(drafted):
+            ids[b, 0] = self.due[b]
+            for i, (token, parent) in enumerate(d):
+                assert -1 <= parent < i, "a draft follows an earlier one"
+                ids[b, i + 1], parents[b, i + 1], depth[b, i + 1] = token, parent + 1, depth[b, parent + 1] + 1
+                if targets[b, parent + 1] < 0:
+                    targets[b, parent + 1] = token
+            at = self.context[b] + np.arange(counts[b])
+            slots[b, :counts[b]] = self.tables[b, at // bs].astype(np.int64) * bs + at % bs
+        put = lambda name, a: self.prog.set_input(self.dg.inputs[name], a)  # noqa: E731
+        put("ids", ids)
+        put("pos", (self.context[:, None] + depth).astype(np.int32))
+        put("context", self.context)
+        put("counts", counts)
+        put("parents", parents)
+        put("slots", slots.view(np.int32))
+        put("targets", targets)
+        self.prog.run()
+        follows = self.prog.read(self.dg.token).reshape(B, D).astype(np.int64)
+        path, gained = np.zeros((B, D), np.int32), []
+        kept = np.ones(B, np.int32)
+        for b in range(B):
+            at, new = 0, [int(follows[b, 0])]
+            for i in range(1, int(counts[b])):      # drafts come behind their parents
+                if parents[b, i] == at and ids[b, i] == new[-1]:
+                    at = path[b, kept[b]] = i
+                    kept[b] += 1
+                    new.append(int(follows[b, i]))
+            gained.append(new)
+        self._keep(path, kept)
+        self.context = self.context + kept
+        self.due = np.array([n[-1] for n in gained], np.int32)
+        self.steps += 1
+        return gained
+
+    def _keep(self, path: np.ndarray, kept: np.ndarray) -> None:
+        from . import device_ops as ops
+
+        cfg, B, D, n = self.cfg, self.batch, self.drafts, self.tables.size
+        self.room.write(4 * n, np.concatenate([self.context, kept, path.reshape(-1)]).astype(np.int32))
+        base = self.room.device_ptr
+        ints = lambda at, shape: ops.DeviceArray(base + 4 * at, shape, "<i4", owner=self.room)  # noqa: E731
+        offs, page = self.native.state_offsets, cfg.n_kv_heads * cfg.block_size * cfg.head_dim * 2
+        step = offs[2] - offs[0] if cfg.n_layers > 1 else page * self.pool_blocks
+        row = cfg.head_dim * 2
+        pool = lambda off: ops.DeviceArray(self.native.state.device_ptr + off, (cfg.n_layers, self.pool_blocks, cfg.n_kv_heads, cfg.block_size, cfg.head_dim), "<f2",  # noqa: E731
+                                           (step, page, cfg.block_size * row, row, 2), self.native.state)
+        status = 2 * B + B * D + n
+        ops.cache_keep(self.native, pool(offs[0]), pool(offs[1]), ints(0, self.tables.shape), ints(n, (B,)), ints(n + 2 * B, (B, D)), ints(n + B, (B,)),
+                       status=ints(status, (1,)))
+        if int(self.room.read(4 * status, 4).view(np.int32)[0]):     # waits for the stream
+            raise RuntimeError("a block table holds a page outside the pools")
+
+    def scores(self) -> np.ndarray:
+        """Of the last pass, per sequence and row (the token that was due, then its drafts): the log probability of the first draft that follows it (0:
+        none does), the entropy of what may follow, ids and log probabilities of the alternatives (``Graph.token_logprobs``)."""
+        return self.prog.read(self.dg.extras["scores"]).reshape(self.batch, self.drafts, -1)
+
+    def logits(self) -> np.ndarray:
+        return self.prog.read(self.dg.logits).reshape(self.batch, self.drafts, -1)
+
+    def free(self) -> None:
+        self.prog.free()
+        self.room.free()
