@@ -130,13 +130,13 @@ __global__ void __launch_bounds__(128) k_serve_attn_any(const ServeAttn a) {
 const char *serve_attn_refusal(const ServeAttn &a) {
     if (a.hs < 8 || a.hs > 512 || a.hs % 8) return "the head size must be a multiple of 8 up to 512";
     if (a.kv_heads < 1 || a.heads < 1 || a.heads % a.kv_heads || a.heads > 65535) return "the query heads must be a multiple of the kv heads";
-    if (a.seqs < 0 || a.q_rows < 0 || a.q_rows > 0x7fffffff || a.kv_rows < 0 || a.kv_rows > 0x7fffffff) return "more than 2^31 - 1 rows";
+    if (a.seqs < 0 || a.seqs > 0x7fffff00 || a.q_rows < 0 || a.q_rows > 0x7fffff00 || a.kv_rows < 0 || a.kv_rows > 0x7fffff00) return "more than 2^31 - 256 rows";
     if (!(a.scale > 0.f) || a.scale > 3e38f) return "the scale must be positive and finite";
     if (a.paged) {
         if (a.bf16) return "the cache holds f16";
         if (a.drafts < 1 || a.drafts > TREE_MAX_DRAFTS) return "1 to 64 drafted tokens per sequence";
         if (a.block_size < 1 || (a.block_size & (a.block_size - 1)) || a.max_blocks < 1) return "the block size must be a power of two";
-        if ((int64_t)a.max_blocks * a.block_size > 0x7fffffff) return "block tables of more than 2^31 - 1 tokens";
+        if ((int64_t)a.max_blocks * a.block_size > 0x7fffff00) return "block tables of more than 2^31 - 256 tokens";
         if (a.pool_blocks < 0 || a.pool_blocks > 0x7fffffff) return "pools of more than 2^31 - 1 pages";
     }
     return nullptr;

@@ -19,8 +19,8 @@
 // are read on the device, so the same launch serves any batch.
 //
 // Tiles at the diagonal, at the end of a sequence or in the tree are `special`: scores are masked by index, and because 0 x NaN is not 0,
-// two warps look through their values first: rows behind the sequence's end become zero, and where a value is not finite the rows of the
-// tile are summed key by key instead (attn_slow).
+// a warp looks through their values first: rows behind the sequence's end become zero, and so do values that are not finite, which the rows that see
+// them get added afterwards (add_odd_values).
 //
 // Every wait is bounded (tc_common.cuh); one that gives up sets the status word to 2.
 #include <algorithm>
@@ -44,7 +44,7 @@ constexpr int T = 128;
 constexpr int THREADS = 384;            // warp 0 shares out the work and copies queries and keys, 3 values, 1 issues MMAs, 2 looks through special tiles, 4-7 and 8-11 are the streams
 constexpr float RESCALE_STEP = 8.f;     // in the base-2 domain
 constexpr uint32_t O_COL = 256;         // S / P of stream x at column 128 x, O at 256 + 128 x
-constexpr int SLOW_RING = 16;
+constexpr int ODD_RING = 16;
 constexpr int REGS_ROLES = 88, REGS_STREAMS = 200;   // registers of a thread (setmaxnreg): the streams hold a row of 128 scores
 
 // Keys of a tile. 64 without SHARE: a tile of values is held for a shorter time and more of them are on their way in the same room
@@ -386,24 +386,11 @@ __device__ __forceinline__ void turn4(uint4 (&w)[4]) {
     swap(w[1], w[3], 2);
 }
 
-// ---- a row whose segment has a special tile with values that are not finite: key by key in f32, one thread per row
-template <typename E, bool PAGED>
-__device__ __noinline__ float slow_score(const ServeAttn &a, const ServeSeq &sq, int seq, int kvh, const char *q, int key) {
-    const ServeRow at = serve_kv_row<PAGED>(a, seq, sq, kvh, key);
-    float s = 0.f;
-    if (!at.k) return -CUDART_INF_F;
-    for (int c = 0; c < a.hs / 8; c++) {
-        float x[8], y[8];
-        serve_unpack<E>(*reinterpret_cast<const uint4 *>(q + c * 16), x);
-        serve_unpack<E>(*reinterpret_cast<const uint4 *>(at.k + c * 16), y);
-#pragma unroll
-        for (int e = 0; e < 8; e++) s = fmaf(x[e], y[e], s);
-    }
-    return s;
-}
-// part: null where the segment is a whole row tile, else where its (m, l) and sums go (rows of them)
+// ---- values of special tiles that are not finite, added to the results of a row that sees them (they were zero in the product)
+// part: null where the segment is a whole row tile and its results lie in `out` already divided (inv), else its sums (rows of them); m: what the
+// exponents refer to
 template <typename E, bool PAGED, int KT>
-__device__ __noinline__ void slow_row(const Params &p, const Segment &g, RowView v, int token, int head, float *part, int rows, int prow) {
+__device__ __noinline__ void add_odd_values(const Params &p, const Segment &g, RowView v, int token, int head, float m, float inv, float *part, int rows, int prow) {
     ServeSeq sq;
     sq.q0 = g.q0;
     sq.k0 = g.k0;
@@ -411,42 +398,27 @@ __device__ __noinline__ void slow_row(const Params &p, const Segment &g, RowView
     sq.nk = g.nk;
     sq.ok = true;
     const char *q = (const char *)p.a.q + (int64_t)(g.q0 + token) * p.a.q_stride + (int64_t)head * p.a.hs * 2;
-    char *dst = (char *)p.a.out + (int64_t)(g.q0 + token) * p.a.out_stride + (int64_t)head * p.a.hs * 2;
-    const int ctx = g.ctx(), k0 = g.t0 * KT, k1 = min((int64_t)g.nk, (int64_t)g.t1 * KT);
-    float m = -CUDART_INF_F, l = 0.f;
-    for (int key = k0; key < k1; key++)
-        if (sees<PAGED>(v, ctx, key)) m = fmaxf(m, slow_score<E, PAGED>(p.a, sq, g.seq, g.kvh, q, key) * p.scale_log2);
-    if (m == -CUDART_INF_F) m = 0.f;
-    for (int key = k0; key < k1; key++)
-        if (sees<PAGED>(v, ctx, key)) l += ex2(slow_score<E, PAGED>(p.a, sq, g.seq, g.kvh, q, key) * p.scale_log2 - m);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (part) {
-        part[prow * 2] = m;
-        part[prow * 2 + 1] = l;
-    }
-    for (int c0 = 0; c0 < p.a.hs; c0 += 8) {
-        float o[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = 0.f;
-        for (int key = k0; key < k1; key++) {
-            if (!sees<PAGED>(v, ctx, key)) continue;
-            const ServeRow at = serve_kv_row<PAGED>(p.a, g.seq, sq, g.kvh, key);
-            if (!at.v) continue;
-            const float w = ex2(slow_score<E, PAGED>(p.a, sq, g.seq, g.kvh, q, key) * p.scale_log2 - m);
-            float y[8];
-            serve_unpack<E>(*reinterpret_cast<const uint4 *>(at.v + c0 * 2), y);
-#pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = fmaf(w, y[e], o[e]);
-        }
-        if (part) {
-            float4 *at = reinterpret_cast<float4 *>(part + rows * 2) + (size_t)(c0 / 4) * rows + prow;
-            at[0] = make_float4(o[0], o[1], o[2], o[3]);
-            at[rows] = make_float4(o[4], o[5], o[6], o[7]);
-        } else {
-            E r[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) r[e] = serve_round<E>(o[e] * inv);
-            *reinterpret_cast<uint4 *>(dst + c0 * 2) = *reinterpret_cast<const uint4 *>(r);
+    E *dst = reinterpret_cast<E *>((char *)p.a.out + (int64_t)(g.q0 + token) * p.a.out_stride) + (int64_t)head * p.a.hs;
+    const int ctx = g.ctx(), k1 = (int)min((int64_t)g.nk, (int64_t)g.t1 * KT);
+    for (int key = max(g.t0, g.special) * KT; key < k1; key++) {
+        if (!sees<PAGED>(v, ctx, key)) continue;
+        const ServeRow at = serve_kv_row<PAGED>(p.a, g.seq, sq, g.kvh, key);
+        if (!at.v) continue;
+        float weight = -1.f;   // worked out at the first value of the key
+        for (int c = 0; c < p.a.hs; c++) {
+            const float y = (float)reinterpret_cast<const E *>(at.v)[c];
+            if (fabsf(y) < CUDART_INF_F) continue;
+            if (weight == -1.f) {
+                float s = 0.f;
+                for (int d = 0; d < p.a.hs; d++) s = fmaf((float)reinterpret_cast<const E *>(q)[d], (float)reinterpret_cast<const E *>(at.k)[d], s);
+                weight = ex2(s * p.scale_log2 - m) * inv;
+            }
+            if (part) {
+                float *o = part + rows * 2 + ((size_t)(c / 4) * rows + prow) * 4 + c % 4;
+                *o = fmaf(weight, y, *o);
+            } else {
+                dst[c] = serve_round<E>(fmaf(weight, y, (float)dst[c]));
+            }
         }
     }
 }
@@ -466,7 +438,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     __shared__ uint64_t bar_q, bar_qfree, bar_k[NS], bar_kfree[NS], bar_v[NS], bar_vfree[NS], bar_fix[NS], bar_s[2], bar_p[2], bar_o[2], bar_od;
     __shared__ uint32_t tmem_base_s;
     __shared__ int s_fail;
-    __shared__ volatile int slow_ring[SLOW_RING];   // segment + 1 of those whose special tiles hold values that are not finite
+    __shared__ volatile int odd_ring[ODD_RING];   // segment + 1 of those whose special tiles hold values that are not finite
     __shared__ Segment segs[SEG_RING];
     __shared__ uint64_t bar_seg[SEG_RING], bar_segfree[SEG_RING];
     __shared__ float pair_ml[2][T][2];
@@ -495,7 +467,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             mbar_init(&bar_segfree[i], 11);   // every warp but the one that writes
         }
         s_fail = 0;
-        for (int i = 0; i < SLOW_RING; i++) slow_ring[i] = 0;
+        for (int i = 0; i < ODD_RING; i++) odd_ring[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) tmem_alloc(&tmem_base_s, 512);
@@ -714,7 +686,11 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                             odd |= ((w.x & EXP) + ONE) | ((w.y & EXP) + ONE) | ((w.z & EXP) + ONE) | ((w.w & EXP) + ONE);
                         }
                     }
-                    if (odd & 0x80008000u) slow_ring[seg % SLOW_RING] = seg + 1;
+                    if (__any_sync(0xffffffffu, odd & 0x80008000u)) {
+                        odd_ring[seg % ODD_RING] = seg + 1;
+                        uint32_t *e = reinterpret_cast<uint32_t *>(v);
+                        for (int i = lane; i < TILE / 4; i += 32) e[i] &= ~((((e[i] & EXP) + ONE) >> 15 & 0x00010001u) * 0xffffu);
+                    }
                 }
                 if (j >= g.special) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -829,15 +805,11 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             if (mine > 0) mbar_wait_nap(&bar_o[x], (done[x] - 1) & 1u, fail, 0);
             if (!SHARE && other > 0) mbar_wait_nap(&bar_o[x ^ 1], (done[x ^ 1] - 1) & 1u, fail, 0);
             tc_fence_after();
-            const bool slow = n > 0 && slow_ring[seg % SLOW_RING] == seg + 1;
+            const bool odd = n > 0 && odd_ring[seg % ODD_RING] == seg + 1;
             const bool whole = g.t0 == 0 && g.t1 == g.n;
             float *part = whole ? nullptr : p.partial + ((size_t)blockIdx.x * 2 + (g.t0 > 0 ? 0 : 1)) * (NQ * T) * (2 + HSP);
             const int prow = (SHARE ? x * T : 0) + row;
-            if (slow) {
-                if (PAGED && !have_bits) view.bits = ancestors_of(parents, token & 63, p.a.err);
-                if (live_row && (SHARE || x == 0)) slow_row<E, PAGED, KT>(p, g, view, token, head, part, NQ * T, prow);
-                __syncwarp();
-            } else {
+            {
                 float f_mine = 1.f, f_other = 0.f;
                 if (!SHARE) {
                     pair_ml[x][row][0] = have_ref ? m_ref : -CUDART_INF_F;
@@ -913,6 +885,14 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
 #pragma unroll
                         for (int e = 0; e < 8; e++) to[e * NQ * T] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                     }
+                }
+                if (odd) {
+                    // the rows' results, some of them written by other lanes or (halves of the columns) the other stream's warps, are all there
+                    if (SHARE) __syncwarp();
+                    else asm volatile("bar.sync 1, 256;" ::: "memory");
+                    if (PAGED && !have_bits) view.bits = ancestors_of(parents, token & 63, p.a.err);
+                    if (view.lim >= 0 && (SHARE || x == 0)) add_odd_values<E, PAGED, KT>(p, g, view, token, head, m_ref, whole ? inv : 1.f, part, NQ * T, prow);
+                    __syncwarp();
                 }
             }
             tc_fence_before();

@@ -1065,6 +1065,8 @@ void lower_serve_attn(L &l) {
     Place p[7], ps;
     for (int i = 0; i < 7; i++)
         if (t.src[i] >= 0) p[i] = l.place(t.src[i]);
+    for (int i = 0; i < 3; i++)
+        if (p[i].off % 16) unsupported(t, "queries, keys and values must start on 16-byte boundaries");
     const bool own_kv_off = t.src[4] >= 0;
     if (serve_attn_scratch_bytes(a, sm) > 0) {
         const int64_t sc = l.c.layout->scratch[l.pos];

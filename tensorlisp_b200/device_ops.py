@@ -52,9 +52,11 @@ def _code(dtype) -> int:
 
 
 def _view(native, x, name: str, types, ndim: int):
-    """(address, ggml type, shape, strides in elements) of an array of one of `types` with `ndim` dimensions on the handle's device."""
+    """(address, ggml type, shape, strides in elements, whether it is known to be dense) of an array of one of `types` with `ndim` dimensions on the
+    handle's device."""
+    dense = False
     if hasattr(x, "data_ptr"):
-        code, shape, strides, ptr = _dtypes.get(x.dtype) or _code(x.dtype), x.shape, x.stride(), x.data_ptr()
+        code, shape, strides, ptr, dense = _dtypes.get(x.dtype) or _code(x.dtype), x.shape, x.stride(), x.data_ptr(), x.is_contiguous()
         if x.get_device() != native.ordinal:
             _invalid("%s lies on another device than the handle's (GPU %d)" % (name, native.ordinal))
     else:
@@ -76,13 +78,13 @@ def _view(native, x, name: str, types, ndim: int):
         _invalid("%s must be %s" % (name, " or ".join(_NAMES[t] for t in types)))
     if len(shape) != ndim:
         _invalid("%s must have %d dimensions, got %d" % (name, ndim, len(shape)))
-    return ptr, code, shape, strides
+    return ptr, code, shape, strides, dense
 
 
 def _dense(view, name: str, first: int = 0) -> None:
     """Dimensions from `first` on are dense."""
-    _, _, shape, strides = view
-    if 0 in shape:
+    _, _, shape, strides, dense = view
+    if dense or 0 in shape:
         return
     n = 1
     for i in range(len(shape) - 1, first - 1, -1):
@@ -115,7 +117,7 @@ def _given(x, name: str):
 
 def _step(view) -> int:
     """Bytes from row to row; those of a dense row where there are not two."""
-    _, code, shape, strides = view
+    _, code, shape, strides, _ = view
     if shape[0] > 1:
         return strides[0] * _SIZE[code]
     n = _SIZE[code]
@@ -127,7 +129,7 @@ def _step(view) -> int:
 def _room(native, workspace) -> tuple:
     if workspace is None:
         return 0, 0
-    ptr, code, shape, _ = v = _view(native, workspace, "workspace", _ROOM, 1)
+    ptr, code, shape, _, _ = v = _view(native, workspace, "workspace", _ROOM, 1)
     _dense(v, "workspace")
     return ptr, shape[0] * _SIZE[code]
 
