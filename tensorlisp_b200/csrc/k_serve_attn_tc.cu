@@ -47,13 +47,18 @@ constexpr uint32_t O_COL = 256;         // S / P of stream x at column 128 x, O 
 constexpr int ODD_RING = 16;
 constexpr int REGS_ROLES = 88, REGS_STREAMS = 200;   // registers of a thread (setmaxnreg): the streams hold a row of 128 scores
 
-// Keys of a tile. 64 without SHARE: a tile of values is held for a shorter time and more of them are on their way in the same room
-__host__ __device__ constexpr int key_tile(bool share) { return share ? 128 : 64; }
+// Keys of a tile. 64 without SHARE: a tile of values is held for a shorter time and more of them are on their way in the same room. With SHARE an MMA
+// takes 60 to 75 cycles whether it has 64 keys or 128, so head size 128 takes 128
+__host__ __device__ constexpr int key_tile(int hsp, bool share) { return share && hsp == 128 ? 128 : 64; }
+// Tiles of S (and the P written over it) that a stream has in tensor memory. Two of them keep a stream's exponentials going while the tile in front is
+// multiplied: 24 prompts of up to 1000 tokens, 16 heads of 64, 64 us against 74 with one tile of 128 keys. Heads of 128 have room for two only of 64 keys: 1 x 8192
+// 531 us against 490
+__host__ __device__ constexpr int buffers(int hsp, bool share) { return share && hsp == 64 ? 2 : 1; }
 // What a row tile costs beside its key tiles, in key tiles, and with it a CTA's least share. us with 1, 2, 4, 6: 1 x 8192 546, 506, 500, 511; tree 48 x 32 over
-// up to 8192 182, 180, 174, 172
-__host__ __device__ constexpr int overhead(int kt) { return kt == 128 ? 3 : 5; }
-__host__ __device__ constexpr int stages(int hsp, bool share) { return hsp == 128 ? (share ? 2 : 6) : (share ? 4 : 8); }
-__host__ __device__ constexpr int smem_bytes(int hsp, bool share) { return ((share ? 2 : 1) * T + 2 * stages(hsp, share) * key_tile(share)) * hsp * 2; }
+// up to 8192 182, 180, 174, 172. With 2, 3, 5, 8: 24 x 1000 of head size 64 63, 60, 62, 66
+constexpr int overhead(bool share) { return share ? 3 : 5; }
+__host__ __device__ constexpr int stages(int hsp, bool share) { return hsp == 128 ? (share ? 2 : 6) : 8; }
+__host__ __device__ constexpr int smem_bytes(int hsp, bool share) { return ((share ? 2 : 1) * T + 2 * stages(hsp, share) * key_tile(hsp, share)) * hsp * 2; }
 
 struct Place {
     int seq, kvh, r;
@@ -65,7 +70,7 @@ struct Params {
     float scale_log2;
     int pool_rows;            // paged: rows of a pool
     int group, tpt, tt;       // heads per KV head; tokens of a row tile; of the row tiles that a unit covers
-    int ctas, min_units;      // a CTA's least share
+    int ctas, overhead, min_units;   // of a row tile; a CTA's least share
     Place *ends;              // [CTA]: where its stretch ends, which tells k_serve_join what it cuts
     float *partial;           // [CTA][2]: (m, l) of the rows, then O as [hsp / 4][rows][4], which the writers' lanes (rows) fill side by side
 };
@@ -101,7 +106,7 @@ __device__ __forceinline__ int key_tiles(const Params &p, const ServeSeq &s, int
 // units of row tiles [0, r)
 template <bool PAGED, int KT>
 __device__ __forceinline__ int64_t units_before(const Params &p, const ServeSeq &s, int r) {
-    int64_t u = (int64_t)r * overhead(KT);
+    int64_t u = (int64_t)r * p.overhead;
     if (PAGED) return u + (int64_t)min(r, (s.nq + p.tt - 1) / p.tt) * ((s.nk + KT - 1) / KT);
     const int R = row_tiles<false>(p, s);
     const int full = min(r, R - 1);
@@ -220,7 +225,7 @@ struct Walk {
                 continue;
             }
             const int n = key_tiles<PAGED, KT>(p, sq, at.r);
-            const int64_t take = min(left, n + overhead(KT) - at.off), off = at.off;
+            const int64_t take = min(left, n + p.overhead - at.off), off = at.off;
             g.seq = at.seq;
             g.kvh = at.kvh;
             g.token0 = at.r * p.tt;
@@ -235,7 +240,7 @@ struct Walk {
             g.special = (PAGED ? g.ctx() : max(0, g.token0 + g.ctx() + 1)) / KT;
             left -= take;
             at.off += take;
-            if (at.off == n + overhead(KT)) {
+            if (at.off == n + p.overhead) {
                 at.off = 0;
                 at.r++;
             }
@@ -429,13 +434,13 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     using namespace tc;
     using namespace sat;
     using E = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-    constexpr int KT = key_tile(SHARE), NS = stages(HSP, SHARE), HALVES = HSP / 64, NQ = SHARE ? 2 : 1;
+    constexpr int BUFS = buffers(HSP, SHARE), KT = key_tile(HSP, SHARE), NS = stages(HSP, SHARE), HALVES = HSP / 64, NQ = SHARE ? 2 : 1;
     constexpr int QTILE = T * HSP * 2, QHALF = T * 128, TILE = KT * HSP * 2, KHALF = KT * 128;   // bytes; halves: 64 columns
     constexpr uint32_t FMT = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(T >> 4) << 24);
     constexpr uint32_t IDESC_QK = FMT | ((uint32_t)(KT >> 3) << 17), IDESC_PV = FMT | (1u << 16) | ((uint32_t)(HSP >> 3) << 17);
     extern __shared__ __align__(1024) uint8_t smem[];   // behind 3 KB of the arrays below, so that three stages fill the 227 KB to the byte
     uint8_t *qs = smem, *ks = qs + NQ * QTILE, *vs = ks + NS * TILE;
-    __shared__ uint64_t bar_q, bar_qfree, bar_k[NS], bar_kfree[NS], bar_v[NS], bar_vfree[NS], bar_fix[NS], bar_s[2], bar_p[2], bar_o[2], bar_od;
+    __shared__ uint64_t bar_q, bar_qfree, bar_k[NS], bar_kfree[NS], bar_v[NS], bar_vfree[NS], bar_fix[NS], bar_s[2][BUFS], bar_p[2][BUFS], bar_o[2][BUFS], bar_od;
     __shared__ uint32_t tmem_base_s;
     __shared__ int s_fail;
     __shared__ volatile int odd_ring[ODD_RING];   // segment + 1 of those whose special tiles hold values that are not finite
@@ -457,9 +462,11 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             mbar_init(&bar_fix[i], 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(&bar_s[i], 1);
-            mbar_init(&bar_p[i], 4);
-            mbar_init(&bar_o[i], 1);
+            for (int b = 0; b < BUFS; b++) {
+                mbar_init(&bar_s[i][b], 1);
+                mbar_init(&bar_p[i][b], 4);
+                mbar_init(&bar_o[i][b], 1);
+            }
         }
         mbar_init(&bar_od, 8);
         for (int i = 0; i < SEG_RING; i++) {
@@ -588,75 +595,70 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         if (lane == 0) p.ends[blockIdx.x] = walk.left == 0 ? walk.at : Place{p.a.seqs, 0, 0, 0};
     } else if (warp == 1) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
-        // ---- MMA issue: step i is stream i & 1; S of step i + 2 follows O of step i, which has read the P that it overwrites
+        // ---- MMA issue: S of a tile follows O of the tile that had its columns, which has read the P that it overwrites. With SHARE streams are constants of the
+        // code: with them taken from a step's number, 1 x 8192 takes 500 us against 483 and 24 x 1000 of head size 64 73 against 64.
         const bool leader = elect_one();
         int tile = 0, seg = 0;
         uint32_t n_p[2] = {0, 0};
         while (next()) {
-            const int n = g.t1 - g.t0, steps = SHARE ? 2 * n : n;
+            const int n = g.t1 - g.t0;
             if (n == 0) continue;
-            auto issue_s = [&](int i) {
-                const int x = i & 1, k = tile + (SHARE ? i >> 1 : i), s = k % NS;
+            auto buffer = [&](int i) { return BUFS == 2 ? (tile + i) & 1 : 0; };
+            auto column = [&](int x, int i) { return (uint32_t)(x * T + buffer(i) * KT); };   // of S and P
+            auto issue_s = [&](int x, int i) {
+                const int s = (tile + i) % NS;
                 tc_fence_after();
                 if (leader) {
 #pragma unroll
                     for (int h = 0; h < HALVES; h++) {
                         const uint64_t qd = plain::desc_sw128(su32(qs + (SHARE ? x * QTILE : 0) + h * QHALF)), kd = plain::desc_sw128(su32(ks + s * TILE + h * KHALF));
 #pragma unroll
-                        for (int e = 0; e < 4; e++) umma_f16(tmem + (uint32_t)(x * T), qd + 2 * e, kd + 2 * e, IDESC_QK, (h | e) ? 1u : 0u);
+                        for (int e = 0; e < 4; e++) umma_f16(tmem + column(x, i), qd + 2 * e, kd + 2 * e, IDESC_QK, (h | e) ? 1u : 0u);
                     }
-                    umma_commit(&bar_s[x]);
-                    if (!SHARE || x == 1) umma_commit(&bar_kfree[s]);
-                    if (i == steps - 1) umma_commit(&bar_qfree);
+                    umma_commit(&bar_s[x][buffer(i)]);
+                    if (!SHARE || x == 1) {
+                        umma_commit(&bar_kfree[s]);
+                        if (i == n - 1) umma_commit(&bar_qfree);
+                    }
                 }
                 __syncwarp();
             };
-            auto issue_o = [&](int i) {
-                const int x = i & 1, s = (tile + (SHARE ? i >> 1 : i)) % NS;
-                if (i == 0 && seg > 0) mbar_wait_nap(&bar_od, (uint32_t)(seg - 1) & 1u, fail, 0);
+            auto issue_o = [&](int x, int i) {
+                const int s = (tile + i) % NS;
+                mbar_wait_nap(&bar_p[x][buffer(i)], (BUFS == 2 ? (uint32_t)(tile + i) >> 1 : n_p[x]) & 1u, fail, 0);
+                if (i == 0 && x == 0 && seg > 0) mbar_wait_nap(&bar_od, (uint32_t)(seg - 1) & 1u, fail, 0);
                 tc_fence_after();
                 if (leader) {
                     const uint64_t vd = desc_mn<KHALF>(su32(vs + s * TILE));
 #pragma unroll
                     for (int e = 0; e < KT / 16; e++)
-                        umma_f16_ta(tmem + O_COL + (uint32_t)(x * T), tmem + (uint32_t)(x * T + e * 8), vd + (uint64_t)(e * 128), IDESC_PV, (i > 1 || e) ? 1u : 0u);
-                    umma_commit(&bar_o[x]);
+                        umma_f16_ta(tmem + O_COL + (uint32_t)(x * T), tmem + column(x, i) + (uint32_t)(e * 8), vd + (uint64_t)(e * 128), IDESC_PV, (i > (SHARE ? 0 : 1) || e) ? 1u : 0u);
+                    umma_commit(&bar_o[x][buffer(i)]);
                     if (!SHARE || x == 1) umma_commit(&bar_vfree[s]);
                 }
                 __syncwarp();
                 n_p[x]++;
             };
-            auto k_bar = [&](int i) { return &bar_k[(tile + (SHARE ? i >> 1 : i)) % NS]; };
-            auto v_bar = [&](int i) { return &bar_fix[(tile + (SHARE ? i >> 1 : i)) % NS]; };
-            auto parity = [&](int i) { return (uint32_t)((tile + (SHARE ? i >> 1 : i)) / NS) & 1u; };
+            auto wait_for = [&](uint64_t *bar, int i) { mbar_wait_nap(&bar[(tile + i) % NS], (uint32_t)((tile + i) / NS) & 1u, fail, 0); };
             mbar_wait_nap(&bar_q, (uint32_t)seg & 1u, fail, 0);
-            if (SHARE) {
-                mbar_wait_nap(k_bar(0), parity(0), fail, 0);
-                issue_s(0);
-                issue_s(1);
-                for (int i = 0; i < steps; i++) {
-                    if ((i & 1) == 0) mbar_wait_nap(v_bar(i), parity(i), fail, 0);
-                    mbar_wait_nap(&bar_p[i & 1], n_p[i & 1] & 1u, fail, 0);
-                    issue_o(i);
-                    if (i + 2 < steps) {
-                        if ((i & 1) == 0) mbar_wait_nap(k_bar(i + 2), parity(i + 2), fail, 0);
-                        issue_s(i + 2);
-                    }
+            // (taking a P that is ready before keys that are not, so that a tile of values is free sooner: 185 us against 177 at 48 x 4096)
+            constexpr int AHEAD = SHARE ? BUFS : 2;
+            for (int i = 0; i < min(AHEAD, n); i++) {
+                wait_for(bar_k, i);
+                issue_s(SHARE ? 0 : i, i);
+                if (SHARE) issue_s(1, i);
+            }
+            for (int i = 0; i < n; i++) {
+                const bool more = i + AHEAD < n;
+                wait_for(bar_fix, i);
+                issue_o(SHARE ? 0 : i & 1, i);
+                if (more) {
+                    wait_for(bar_k, i + AHEAD);
+                    issue_s(SHARE ? 0 : i & 1, i + AHEAD);
                 }
-            } else {
-                // (taking a P that is ready before keys that are not, so that a tile of values is free sooner: 185 us against 177 at 48 x 4096)
-                for (int i = 0; i < min(2, steps); i++) {
-                    mbar_wait_nap(k_bar(i), parity(i), fail, 0);
-                    issue_s(i);
-                }
-                for (int i = 0; i < steps; i++) {
-                    mbar_wait_nap(v_bar(i), parity(i), fail, 0);
-                    mbar_wait_nap(&bar_p[i & 1], n_p[i & 1] & 1u, fail, 0);
-                    issue_o(i);
-                    if (i + 2 < steps) {
-                        mbar_wait_nap(k_bar(i + 2), parity(i + 2), fail, 0);
-                        issue_s(i + 2);
-                    }
+                if (SHARE) {
+                    issue_o(1, i);
+                    if (more) issue_s(1, i + AHEAD);
                 }
             }
             tile += n;
@@ -726,11 +728,12 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             bool have_ref = false;
             for (int i = 0; i < mine; i++) {
                 const int j = g.t0 + (SHARE ? i : 2 * i + x);
-                mbar_wait_nap(&bar_s[x], (done[x] + i) & 1u, fail, 0);
+                const uint32_t t = done[x] + i, b = BUFS == 2 ? t & 1u : 0u;   // the stream's tile; its buffer, for the (t / BUFS)th time
+                mbar_wait_nap(&bar_s[x][b], t / BUFS & 1u, fail, 0);
                 tc_fence_after();
                 float y[KT];
 #pragma unroll
-                for (int c = 0; c < KT / 32; c++) ld32(s_at + 32 * c, y + 32 * c);
+                for (int c = 0; c < KT / 32; c++) ld32(s_at + b * KT + 32 * c, y + 32 * c);
                 tmem_ld_wait();
                 if (j >= g.special) {
                     if (PAGED && !have_bits) {
@@ -764,7 +767,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                     m_ref = mx;
                 }
                 if (__any_sync(0xffffffffu, alpha != 1.f)) {   // never on a segment's first tile
-                    mbar_wait_nap(&bar_o[x], (done[x] + i - 1) & 1u, fail, 0);
+                    mbar_wait_nap(&bar_o[x][(t - 1) % BUFS], (t - 1) / BUFS & 1u, fail, 0);
                     tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < HSP / 32; c++) {
@@ -791,19 +794,20 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                         add2(sums[e & 1], a, b);
                         w[e] = round2<BF16>(a, b);
                     }
-                    st32(s_at + 32 * c, w);
+                    st32(s_at + b * KT + 32 * c, w);
                 }
                 l += total2(sums[0], sums[1]);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_p[x]);
+                if (lane == 0) mbar_arrive(&bar_p[x][b]);
             }
             done[x] += mine;
             done[x ^ 1] += other;
             // ---- the segment's result: O / l, or (m, l, O) where the row tile was cut
-            if (mine > 0) mbar_wait_nap(&bar_o[x], (done[x] - 1) & 1u, fail, 0);
-            if (!SHARE && other > 0) mbar_wait_nap(&bar_o[x ^ 1], (done[x ^ 1] - 1) & 1u, fail, 0);
+            const uint32_t last = done[x] - 1;
+            if (mine > 0) mbar_wait_nap(&bar_o[x][last % BUFS], last / BUFS & 1u, fail, 0);
+            if (!SHARE && other > 0) mbar_wait_nap(&bar_o[x ^ 1][0], (done[x ^ 1] - 1) & 1u, fail, 0);
             tc_fence_after();
             const bool odd = n > 0 && odd_ring[seg % ODD_RING] == seg + 1;
             const bool whole = g.t0 == 0 && g.t1 == g.n;
@@ -929,7 +933,7 @@ __global__ void __launch_bounds__(128) k_serve_join(const __grid_constant__ sat:
     const Place v = c ? p.ends[c - 1] : Place{0, 0, 0, 0};
     if (v.off > 0 && v.seq == w.seq && v.kvh == w.kvh && v.r == w.r) return;   // it begins in a stretch in front
     const ServeSeq sq = serve_seq(p.a, w.seq);
-    const int n = key_tiles<PAGED, key_tile(SHARE)>(p, sq, w.r);
+    const int n = key_tiles<PAGED, key_tile(HSP, SHARE)>(p, sq, w.r);
     if (w.off >= n) return;   // all of its key tiles lie in this stretch
     const int parts = 1 + (int)((n - w.off + p.ends[p.ctas].off - 1) / p.ends[p.ctas].off);
     // 32 rows: a lane's row is its own, a warp's columns a quarter of them
@@ -981,26 +985,32 @@ bool serve_attn_tc_supported(const ServeAttn &a) {
     if (a.paged) return a.block_size >= 8 && a.pool_blocks > 0 && a.pool_blocks * a.kv_heads * a.block_size < 0x7fffffff;
     return a.kv_rows > 0;
 }
-// A pair of row tiles per unit where sequences fill them on average.
-static bool sat_share(const ServeAttn &a) { return !a.paged && a.q_rows * (a.heads / a.kv_heads) > (int64_t)a.seqs * sat::T; }
+// A pair of row tiles per unit where sequences fill more than one on average. While a pair takes a whole sequence, only if the pairs' key tiles are more than the
+// SMs. us with pairs and without, 32 + 8 heads of 128: 1 x 37 tokens 10.0, 8.8; 8 x 40 12.9, 10.9; 64 x 60 31.6, 34.6; 8 x 40 behind 4000 39, 44; 1 x 100 (two pairs
+// a head) 11.4, 13.7; 64 x 100 53, 70
+static bool sat_share(const ServeAttn &a, int sm_count) {
+    const int64_t rows = a.q_rows * (a.heads / a.kv_heads), tile = (int64_t)a.seqs * sat::T;
+    return !a.paged && rows > tile && (rows > 2 * tile || (a.kv_rows + tile - 1) / tile * a.seqs * a.kv_heads > sm_count);
+}
+static int sat_padded(const ServeAttn &a) { return a.hs <= 64 ? 64 : 128; }
 static int64_t most_key_tiles(const ServeAttn &a, int kt) { return ((a.paged ? (int64_t)a.max_blocks * a.block_size : a.kv_rows) + kt - 1) / kt; }
 static int sat_ctas(const ServeAttn &a, int sm_count) {
-    const bool share = sat_share(a);
+    const bool share = sat_share(a, sm_count);
     const int64_t tt = (int64_t)(sat::T / (a.heads / a.kv_heads)) * (share ? 2 : 1);
     const int64_t tiles = a.paged ? (a.drafts + tt - 1) / tt * a.seqs : a.q_rows / tt + a.seqs;
-    const int64_t kt = sat::key_tile(share), keys = most_key_tiles(a, (int)kt);
-    const double units = (double)tiles * a.kv_heads * (double)(keys + sat::overhead((int)kt)), least = 1 + sat::overhead((int)kt);
+    const int64_t kt = sat::key_tile(sat_padded(a), share), keys = most_key_tiles(a, (int)kt);
+    const double units = (double)tiles * a.kv_heads * (double)(keys + sat::overhead(share)), least = 1 + sat::overhead(share);
     return units / least < sm_count ? std::max(1, (int)(units / least + 1)) : sm_count;
 }
 static uint64_t sat_ends_bytes(int ctas) { return ((uint64_t)(ctas + 1) * sizeof(sat::Place) + 255) / 256 * 256; }   // the last one: the size of a share
 uint64_t serve_attn_tc_scratch_bytes(const ServeAttn &a, int sm_count) {
     const uint64_t ctas = (uint64_t)sat_ctas(a, sm_count);
-    return sat_ends_bytes((int)ctas) + ctas * 2 * (sat_share(a) ? 2 : 1) * sat::T * (2 + (a.hs <= 64 ? 64 : 128)) * 4;
+    return sat_ends_bytes((int)ctas) + ctas * 2 * (sat_share(a, sm_count) ? 2 : 1) * sat::T * (2 + sat_padded(a)) * 4;
 }
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
 static cudaError_t sat_launch(const sat::Params &p, int ctas, cudaStream_t st) {
     cudaError_t e = launch_pdl(k_serve_attn_tc<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas), dim3(sat::THREADS), sat::smem_bytes(HSP, SHARE), st, p);
-    if (e == cudaSuccess && ctas > 1 && most_key_tiles(p.a, sat::key_tile(SHARE)) > 1)   // a single key tile is never cut
+    if (e == cudaSuccess && ctas > 1 && most_key_tiles(p.a, sat::key_tile(HSP, SHARE)) > 1)   // a single key tile is never cut
         e = launch_pdl(k_serve_join<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas - 1, (SHARE ? 2 : 1) * sat::T / 32), dim3(128), 0, st, p);
     return e;
 }
@@ -1030,9 +1040,11 @@ cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.group = a.heads / a.kv_heads;
     p.tpt = T / p.group;
-    const bool share = sat_share(a);
+    const bool share = sat_share(a, sm_count);
     p.tt = p.tpt * (share ? 2 : 1);
-    p.min_units = 1 + overhead(key_tile(share));
+    const int kt = key_tile(sat_padded(a), share);
+    p.overhead = overhead(share);
+    p.min_units = 1 + p.overhead;
     const uint64_t hs = (uint64_t)a.hs;
     cudaError_t e;
     {
@@ -1040,17 +1052,16 @@ cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count
         const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)p.tpt};
         e = tc_encode_sw128(&p.q, a.q, 3, dims, strides, box, a.bf16);
     }
-    const uint32_t kt = (uint32_t)key_tile(share);
     for (int i = 0; i < 2 && e == cudaSuccess; i++) {
         if (a.paged) {
             p.pool_rows = (int)(a.pool_blocks * a.kv_heads * a.block_size);
             const uint64_t dims[2] = {hs, (uint64_t)p.pool_rows}, strides[1] = {hs * 2};
-            const uint32_t box[2] = {64, std::min((uint32_t)a.block_size, kt)};
+            const uint32_t box[2] = {64, (uint32_t)std::min(a.block_size, kt)};
             e = tc_encode_sw128(i ? &p.v : &p.k, i ? a.v : a.k, 2, dims, strides, box, false);
             continue;
         }
         const uint64_t dims[3] = {hs, (uint64_t)a.kv_heads, (uint64_t)a.kv_rows}, strides[2] = {hs * 2, (uint64_t)(i ? a.v_stride : a.k_stride)};
-        const uint32_t box[3] = {64, 1, kt};
+        const uint32_t box[3] = {64, 1, (uint32_t)kt};
         e = tc_encode_sw128(i ? &p.v : &p.k, i ? a.v : a.k, 3, dims, strides, box, a.bf16);
     }
     if (e != cudaSuccess) return e;
