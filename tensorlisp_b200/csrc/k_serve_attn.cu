@@ -131,7 +131,7 @@ const char *serve_attn_refusal(const ServeAttn &a) {
     if (a.hs < 8 || a.hs > 512 || a.hs % 8) return "the head size must be a multiple of 8 up to 512";
     if (a.kv_heads < 1 || a.heads < 1 || a.heads % a.kv_heads || a.heads > 65535) return "the query heads must be a multiple of the kv heads";
     if (a.seqs < 0 || a.seqs > 0x7fffff00 || a.q_rows < 0 || a.q_rows > 0x7fffff00 || a.kv_rows < 0 || a.kv_rows > 0x7fffff00) return "more than 2^31 - 256 rows";
-    if (!(a.scale > 0.f) || a.scale > 3e38f) return "the scale must be positive and finite";
+    if (!(a.scale > 0.f) || a.scale > 1e38f) return "the scale must be positive and finite";
     if (a.paged) {
         if (a.bf16) return "the cache holds f16";
         if (a.drafts < 1 || a.drafts > TREE_MAX_DRAFTS) return "1 to 64 drafted tokens per sequence";

@@ -1067,6 +1067,8 @@ void lower_serve_attn(L &l) {
         if (t.src[i] >= 0) p[i] = l.place(t.src[i]);
     for (int i = 0; i < 3; i++)
         if (p[i].off % 16) unsupported(t, "queries, keys and values must start on 16-byte boundaries");
+    for (int i = 3; i < 7; i++)
+        if (t.src[i] >= 0 && p[i].off % 4) unsupported(t, "numbers must lie on 4-byte boundaries");
     const bool own_kv_off = t.src[4] >= 0;
     if (serve_attn_scratch_bytes(a, sm) > 0) {
         const int64_t sc = l.c.layout->scratch[l.pos];
@@ -1132,6 +1134,7 @@ void lower_logprobs(L &l) {
     const bool has_tokens = t.src[1] >= 0;
     if (has_tokens) pt = l.place(t.src[1]);
     const Place px = l.place(t.src[0]), pd = l.place(l.id);
+    if (px.off % type_traits(a.type)->size || (has_tokens && pt.off % 4)) unsupported(t, "logits and tokens must be aligned to their values");
     l.push([=](const RunCtx &r) {
         Logprobs x = a;
         float *o = (float *)r.at(pd);

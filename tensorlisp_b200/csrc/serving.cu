@@ -28,6 +28,26 @@ bool overlap(const void *p, uint64_t n, const void *q, uint64_t m) {
     const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
     return p && q && n && m && a < b + m && b < a + n;
 }
+struct Range {
+    const void *p;
+    uint64_t n;
+};
+// what a call writes shares no byte with anything else of it
+bool clash(std::initializer_list<Range> writes, std::initializer_list<Range> reads) {
+    for (const Range *w = writes.begin(); w != writes.end(); w++) {
+        for (const Range *x = w + 1; x != writes.end(); x++)
+            if (overlap(w->p, w->n, x->p, x->n)) return true;
+        for (const Range &r : reads)
+            if (overlap(w->p, w->n, r.p, r.n)) return true;
+    }
+    return false;
+}
+bool numbers(std::initializer_list<const void *> arrays) {
+    for (const void *p : arrays)
+        if (!aligned(p, 4)) return false;
+    return true;
+}
+const char *const NUMBERS = "numbers must lie on 4-byte boundaries", *const CLASH = "a result or the workspace overlaps another array";
 uint64_t span(uint64_t rows, uint64_t stride, uint64_t row) { return rows ? (rows - 1) * stride + row : 0; }
 bool product_fits(std::initializer_list<uint64_t> f) {
     unsigned __int128 n = 1;
@@ -141,11 +161,14 @@ tlb_status tlb_packed_attention(tlb_device *dev, const tlb_packed_attention_args
     if (args->q_stride < q_row || args->out_stride < q_row || args->k_stride < kv_row || args->v_stride < kv_row)
         return fail(TLB_INVALID, me + "a row is longer than its stride");
     if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16)) return fail(TLB_INVALID, me + "rows must start on 16-byte boundaries");
-    const uint64_t q_span = span(a.q_rows, args->q_stride, q_row), o_span = span(a.q_rows, args->out_stride, q_row);
-    if (overlap(a.out, o_span, a.q, q_span) || overlap(a.out, o_span, a.k, span(a.kv_rows, args->k_stride, kv_row)) ||
-        overlap(a.out, o_span, a.v, span(a.kv_rows, args->v_stride, kv_row)))
-        return fail(TLB_INVALID, me + "the result overlaps an input");
-    const uint64_t need = serve_attn_scratch_bytes(a, dev->prop.multiProcessorCount);
+    if (!numbers({a.q_off, a.kv_off, a.err})) return fail(TLB_INVALID, me + NUMBERS);
+    for (uint64_t rows : {(uint64_t)a.q_rows, (uint64_t)a.kv_rows})
+        if (!product_fits({rows, std::max({args->q_stride, args->k_stride, args->v_stride, args->out_stride})})) return fail(TLB_INVALID, me + "sizes overflow");
+    const uint64_t need = serve_attn_scratch_bytes(a, dev->prop.multiProcessorCount), off = ((uint64_t)a.seqs + 1) * 4;
+    if (clash({{a.out, span(a.q_rows, args->out_stride, q_row)}, {args->workspace, need}, {a.err, 4}},
+              {{a.q, span(a.q_rows, args->q_stride, q_row)}, {a.k, span(a.kv_rows, args->k_stride, kv_row)}, {a.v, span(a.kv_rows, args->v_stride, kv_row)},
+               {a.q_off, off}, {a.kv_off, off}}))
+        return fail(TLB_INVALID, me + CLASH);
     if (need && (!args->workspace || args->workspace_bytes < need || !aligned(args->workspace, 16)))
         return fail(TLB_INVALID, me + "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed, got " + std::to_string(args->workspace ? args->workspace_bytes : 0));
     OnDevice on(dev->ordinal);
@@ -168,9 +191,11 @@ tlb_status tlb_tree_attention(tlb_device *dev, const tlb_tree_attention_args *ar
     if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16)) return fail(TLB_INVALID, me + "q, out and the pools must start on 16-byte boundaries");
     const uint64_t row = (uint64_t)a.heads * a.hs * 2, page = (uint64_t)a.kv_heads * a.block_size * a.hs * 2;
     if (!product_fits({(uint64_t)a.pool_blocks, page}) || !product_fits({(uint64_t)a.q_rows, row})) return fail(TLB_INVALID, me + "sizes overflow");
-    const uint64_t pool = (uint64_t)a.pool_blocks * page, rows = (uint64_t)a.q_rows * row;
-    if (overlap(a.out, rows, a.q, rows) || overlap(a.out, rows, a.k, pool) || overlap(a.out, rows, a.v, pool)) return fail(TLB_INVALID, me + "the result overlaps an input");
-    const uint64_t need = serve_attn_scratch_bytes(a, dev->prop.multiProcessorCount);
+    if (!numbers({a.tables, a.context, a.counts, a.parents, a.err})) return fail(TLB_INVALID, me + NUMBERS);
+    const uint64_t need = serve_attn_scratch_bytes(a, dev->prop.multiProcessorCount), pool = (uint64_t)a.pool_blocks * page, rows = (uint64_t)a.q_rows * row, n = (uint64_t)a.seqs * 4;
+    if (clash({{a.out, rows}, {args->workspace, need}, {a.err, 4}},
+              {{a.q, rows}, {a.k, pool}, {a.v, pool}, {a.tables, n * (uint64_t)a.max_blocks}, {a.context, n}, {a.counts, n}, {a.parents, n * (uint64_t)a.drafts}}))
+        return fail(TLB_INVALID, me + CLASH);
     if (need && (!args->workspace || args->workspace_bytes < need || !aligned(args->workspace, 16)))
         return fail(TLB_INVALID, me + "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed, got " + std::to_string(args->workspace ? args->workspace_bytes : 0));
     OnDevice on(dev->ordinal);
@@ -194,17 +219,18 @@ tlb_status tlb_cache_keep(tlb_device *dev, const tlb_cache_keep_args *args, void
     const uint64_t pool = p.pool_blocks * page;
     if (!aligned(p.k_pools, 16) || !aligned(p.v_pools, 16) || p.k_layer_stride % 16 || p.v_layer_stride % 16 || p.k_layer_stride >> 46 || p.v_layer_stride >> 46)
         return fail(TLB_INVALID, me + "pools must start on 16-byte boundaries");
-    bool clash = p.layers > 1 && (p.k_layer_stride < pool || p.v_layer_stride < pool);
-    if (!clash && overlap(p.k_pools, span(p.layers, p.k_layer_stride, pool), p.v_pools, span(p.layers, p.v_layer_stride, pool))) {
+    bool both = p.layers > 1 && (p.k_layer_stride < pool || p.v_layer_stride < pool);
+    if (!both && overlap(p.k_pools, span(p.layers, p.k_layer_stride, pool), p.v_pools, span(p.layers, p.v_layer_stride, pool))) {
         // keys and values of the layers in turn: the same step, and room for one beside the other
         const uint64_t step = p.k_layer_stride;
-        clash = p.layers == 1 || step != p.v_layer_stride;
-        if (!clash) {
+        both = p.layers == 1 || step != p.v_layer_stride;
+        if (!both) {
             const uint64_t k = (uintptr_t)p.k_pools % step, v = (uintptr_t)p.v_pools % step, d = v >= k ? v - k : v + step - k;
-            clash = d < pool || step - d < pool;
+            both = d < pool || step - d < pool;
         }
     }
-    if (clash) return fail(TLB_INVALID, me + "two pools overlap");
+    if (both) return fail(TLB_INVALID, me + "two pools overlap");
+    if (!numbers({p.tables, p.context, p.counts, p.path, p.status})) return fail(TLB_INVALID, me + NUMBERS);
     CacheKeep a{};
     a.kpool = p.k_pools;
     a.vpool = p.v_pools;
@@ -242,10 +268,11 @@ tlb_status tlb_token_logprobs(tlb_device *dev, const tlb_token_logprobs_args *ar
     const uint64_t elem = a.type == TLB_TYPE_F32 ? 4 : 2, row = (uint64_t)a.vocab * elem;
     if (!a.logits || (a.top && (!a.top_ids || !a.top_logprobs)) || (a.tokens && !a.logprob)) return fail(TLB_INVALID, me + "null argument");
     if (args->stride % elem || !aligned(a.logits, elem) || args->stride < row || args->stride >> 40) return fail(TLB_INVALID, me + "rows overlap or are not aligned to their values");
-    const uint64_t in = span(a.rows, args->stride, row), n = (uint64_t)a.rows * 4, nk = n * a.top;
-    if (overlap(a.logprob, n, a.logits, in) || overlap(a.entropy, n, a.logits, in) || overlap(a.top_ids, nk, a.logits, in) || overlap(a.top_logprobs, nk, a.logits, in))
-        return fail(TLB_INVALID, me + "a result overlaps the logits");
-    const uint64_t need = logprobs_scratch_bytes(a, dev->prop.multiProcessorCount);
+    if (!numbers({a.tokens, a.logprob, a.entropy, a.top_ids, a.top_logprobs, a.err})) return fail(TLB_INVALID, me + NUMBERS);
+    if (!product_fits({(uint64_t)a.rows, args->stride})) return fail(TLB_INVALID, me + "sizes overflow");
+    const uint64_t need = logprobs_scratch_bytes(a, dev->prop.multiProcessorCount), n = (uint64_t)a.rows * 4, nk = n * a.top;
+    if (clash({{a.logprob, n}, {a.entropy, n}, {a.top_ids, nk}, {a.top_logprobs, nk}, {args->workspace, need}, {a.err, 4}}, {{a.logits, span(a.rows, args->stride, row)}, {a.tokens, n}}))
+        return fail(TLB_INVALID, me + CLASH);
     if (!args->workspace || args->workspace_bytes < need || !aligned(args->workspace, 16))
         return fail(TLB_INVALID, me + "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed, got " + std::to_string(args->workspace ? args->workspace_bytes : 0));
     OnDevice on(dev->ordinal);

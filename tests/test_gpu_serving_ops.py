@@ -648,3 +648,24 @@ def test_nodes_refuse_what_they_do_not_take():
     refused(lambda g: g.token_logprobs(g.input(G.F32, [100, 2], "x"), None, 33), "32")
     refused(lambda g: g.token_logprobs(g.input(G.I32, [100, 2], "x"), None, 3), "f32, f16 or bf16")
     n.close()
+
+
+def test_nodes_refuse_views_between_two_values():
+    n = Native.load([])
+
+    def refused(build, word):
+        g = G.Graph()
+        g.output(build(g))
+        with pytest.raises(TlbError) as e:
+            NativeProgram.compile(n, g)
+        assert e.value.kind == "Unsupported" and word in str(e.value), str(e.value)
+
+    numbers = lambda g, off: g.view(g.input(G.I32, [16], "at"), [3], offset=off)  # noqa: E731
+    rows = lambda g, h, off=0: g.view(g.input(G.F16, [64 * h * 11], "x"), [64, h, 10], 128, 128 * h, offset=off)  # noqa: E731
+    refused(lambda g: g.packed_attention(rows(g, 4, 2), rows(g, 2), rows(g, 2), numbers(g, 0), 0.1), "")
+    refused(lambda g: g.packed_attention(rows(g, 4), rows(g, 2), rows(g, 2, 8), numbers(g, 0), 0.1), "")
+    refused(lambda g: g.packed_attention(rows(g, 4), rows(g, 2), rows(g, 2), numbers(g, 2), 0.1), "4-byte")
+    refused(lambda g: g.packed_attention(rows(g, 4), rows(g, 2), rows(g, 2), numbers(g, 0), 0.1, numbers(g, 6)), "4-byte")
+    refused(lambda g: g.token_logprobs(g.view(g.input(G.F32, [202], "x"), [100, 2], 400, offset=2), None, 3), "aligned")
+    refused(lambda g: g.token_logprobs(g.input(G.F32, [100, 3], "x"), numbers(g, 3), 3), "aligned")
+    n.close()

@@ -150,3 +150,28 @@ def test_arrays_of_the_wrong_kind_are_refused():
 def test_a_cpu_tensor_is_refused():
     import torch
     refused("another device", ops.token_logprobs, torch.zeros(5, 100), None, array(2, (5,), "<f4"))
+
+
+@pytest.mark.parametrize("word,entry,args", [
+    # rows whose distance in memory does not fit 64 bits
+    ("overflow", "tlb_packed_attention", packed(q_rows=2 ** 31 - 512, q_stride=2 ** 39)), ("overflow", "tlb_packed_attention", packed(kv_rows=2 ** 31 - 512, v_stride=2 ** 39)),
+    ("overflow", "tlb_token_logprobs", scores(rows=2 ** 31 - 1, stride=2 ** 39)),
+    # numbers between two places for numbers
+    ("4-byte", "tlb_packed_attention", packed(q_offsets=A[4] + 2)), ("4-byte", "tlb_packed_attention", packed(kv_offsets=A[6] + 1)), ("4-byte", "tlb_packed_attention", packed(status=A[6] + 2)),
+    ("4-byte", "tlb_tree_attention", tree(tables=A[4] + 2)), ("4-byte", "tlb_tree_attention", tree(context=A[5] + 2)), ("4-byte", "tlb_tree_attention", tree(counts=A[6] + 2)),
+    ("4-byte", "tlb_tree_attention", tree(parents=A[7] + 2)), ("4-byte", "tlb_cache_keep", keep(tables=A[4] + 2)), ("4-byte", "tlb_cache_keep", keep(path=A[7] + 2)),
+    ("4-byte", "tlb_cache_keep", keep(counts=A[6] + 2)), ("4-byte", "tlb_cache_keep", keep(context=A[5] + 2)), ("4-byte", "tlb_token_logprobs", scores(tokens=A[1] + 2)),
+    ("4-byte", "tlb_token_logprobs", scores(logprob=A[2] + 2)), ("4-byte", "tlb_token_logprobs", scores(top_ids=A[4] + 2)), ("4-byte", "tlb_token_logprobs", scores(top_logprobs=A[5] + 2)),
+    # results on top of one another, of the numbers that are read, or of the workspace
+    ("overlaps", "tlb_packed_attention", packed(q_offsets=A[3] + 512)), ("overlaps", "tlb_packed_attention", packed(kv_offsets=A[3])), ("overlaps", "tlb_packed_attention", packed(status=A[4] + 8)),
+    ("overlaps", "tlb_tree_attention", tree(tables=A[3])), ("overlaps", "tlb_tree_attention", tree(parents=A[3] + 4096 - 4)), ("overlaps", "tlb_tree_attention", tree(status=A[6] + 4)),
+    ("overlaps", "tlb_token_logprobs", scores(entropy=A[2] + 8)), ("overlaps", "tlb_token_logprobs", scores(top_ids=A[5] + 44)), ("overlaps", "tlb_token_logprobs", scores(logprob=A[1] + 8)),
+    ("overlaps", "tlb_token_logprobs", scores(workspace=A[5] + 32)), ("overlaps", "tlb_token_logprobs", scores(workspace=A[0] + 1184))])
+def test_arrays_in_impossible_places(word, entry, args):
+    call(entry, args, word, "Invalid")
+
+
+def test_results_side_by_side_are_fine():
+    # what a refusal must not take for an overlap: arrays that touch; the refusal that follows is another one
+    call("tlb_token_logprobs", scores(entropy=A[2] + 12, workspace=A[5] + 48, workspace_bytes=16), "workspace of", "Invalid")
+    call("tlb_token_logprobs", scores(tokens=A[2] - 12, workspace_bytes=16), "workspace of", "Invalid")
