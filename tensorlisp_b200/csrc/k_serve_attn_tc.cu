@@ -450,7 +450,6 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     volatile int *fail = &s_fail;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    griddep_launch();
     if (tid == 0) {
         mbar_init(&bar_q, 1);
         mbar_init(&bar_qfree, 1);
@@ -478,14 +477,16 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) tmem_alloc(&tmem_base_s, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // Kernels behind may start only now: one that took this SM's tensor memory first would hold it until this CTA, which would wait for it, is over
+    griddep_launch();
     griddep_wait();
     if (warp == 2 && blockIdx.x == 0 && p.a.err) {
         for (int s = lane; s < p.a.seqs; s += 32)
             if (!serve_seq(p.a, s).ok) report_error(p.a.err, TLB_ERR_INDEX);
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
     const uint32_t tmem = tmem_base_s;
     Segment g;
     int g_at = 0;   // segments seen
