@@ -1,7 +1,7 @@
 // The attention of k_serve_attn.cu on the 5th-generation tensor cores: head sizes up to 128, f16 or bf16.
 //
 // A tile of 128 rows holds `tpt` tokens x the query heads of one KV head (token by token, so a short sequence or a few drafts fill it as
-// well as they can), a key tile 128 keys. Keys and values come by TMA from where they lie (rows of any stride, or pages), 128-byte
+// well as they can), a key tile 64 or 128 keys. Keys and values come by TMA from where they lie (rows of any stride, or pages), 128-byte
 // swizzled; V is read as the MN-major operand, so nothing is packed or transposed first. Columns past the head size and rows past the
 // tensors are filled with zeros by the copy.
 //
@@ -21,6 +21,13 @@
 // Tiles at the diagonal, at the end of a sequence or in the tree are `special`: scores are masked by index, and because 0 x NaN is not 0,
 // a warp looks through their values first: rows behind the sequence's end become zero, and so do values that are not finite, which the rows that see
 // them get added afterwards (add_odd_values).
+//
+// What bounds it. Prompts: a 128 x 128 x 16 MMA takes 60 to 75 cycles to issue and execute, which is 62 % of the time of 1 x 8192 tokens (32 + 8 heads of 128: 480 us,
+// 1.15 PFLOP/s while the clock holds, 970 TFLOP/s under the power cap); the rest is the chain of a stream (read S 250 cycles, maximum 400, exponentials 1400, P V and the
+// next Q K 1024) where the other one does not cover it. Drafts: the keys' and values' bytes, pages of 4 KB in random order: 48 sequences x 32 drafts over up to 8192
+// tokens 166 us = 5.1 TB/s. Short calls: the plan (5000 cycles from the kernel's start to the first copy), an epilogue of 3000 and the joining launch.
+// Polynomials for some of the exponentials (25, 38, 50 %: 500 us -> 527, 555, 622), P handed over in halves (489 -> 500) and P beside S for heads of 64 (74 -> 82)
+// lost.
 //
 // Every wait is bounded (tc_common.cuh); one that gives up sets the status word to 2.
 #include <algorithm>
@@ -51,8 +58,8 @@ constexpr int REGS_ROLES = 88, REGS_STREAMS = 200;   // registers of a thread (s
 // takes 60 to 75 cycles whether it has 64 keys or 128, so head size 128 takes 128
 __host__ __device__ constexpr int key_tile(int hsp, bool share) { return share && hsp == 128 ? 128 : 64; }
 // Tiles of S (and the P written over it) that a stream has in tensor memory. Two of them keep a stream's exponentials going while the tile in front is
-// multiplied: 24 prompts of up to 1000 tokens, 16 heads of 64, 64 us against 74 with one tile of 128 keys. Heads of 128 have room for two only of 64 keys: 1 x 8192
-// 531 us against 490
+// multiplied: 24 prompts of up to 1000 tokens, 16 heads of 64, 62 us against 74 with one tile of 128 keys. Heads of 128 have room for two only of 64 keys: 1 x 8192
+// 531 us against 483
 __host__ __device__ constexpr int buffers(int hsp, bool share) { return share && hsp == 64 ? 2 : 1; }
 // What a row tile costs beside its key tiles, in key tiles, and with it a CTA's least share. us with 1, 2, 4, 6: 1 x 8192 546, 506, 500, 511; tree 48 x 32 over
 // up to 8192 182, 180, 174, 172. With 2, 3, 5, 8: 24 x 1000 of head size 64 63, 60, 62, 66
@@ -921,7 +928,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     if (tid == 0 && s_fail && p.a.err) report_error(p.a.err, 2);
 }
 
-// Row tiles that were cut: CTA (c, rows) adds up the parts of the one that begins in stretch c of the line and reaches over its end.
+// Row tiles that were cut (3 to 9 us beside the launch in front, whose plan it reads): CTA (c, rows) adds up the parts of the one that begins in stretch c of the line and reaches over its end.
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
 __global__ void __launch_bounds__(128) k_serve_join(const __grid_constant__ sat::Params p) {
     using namespace sat;

@@ -669,3 +669,80 @@ def test_nodes_refuse_views_between_two_values():
     refused(lambda g: g.token_logprobs(g.view(g.input(G.F32, [202], "x"), [100, 2], 400, offset=2), None, 3), "aligned")
     refused(lambda g: g.token_logprobs(g.input(G.F32, [100, 3], "x"), numbers(g, 3), 3), "aligned")
     n.close()
+
+
+# ------------------------------------------------------------------------------------------------ far away
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_packed_attention_behind_four_gigabytes(native, D):
+    H, Gr, rows = 4, 2, 1_200_000
+    q_at, kv_at = offsets([30, 70]), offsets([100, 200], rows - 300)
+    wide_q, wide_o = (torch.empty((100, 1 << 25), dtype=torch.float16, device="cuda") for _ in range(2))     # rows 64 MB apart
+    q, out = (x[:, :H * D].view(100, H, D) for x in (wide_q, wide_o))
+    both = torch.empty((rows, 2, 1024), dtype=torch.float16, device="cuda")                                    # 4 KB apart
+    k, v = both[:, 0, :Gr * D].unflatten(1, (Gr, D)), both[:, 1, :Gr * D].unflatten(1, (Gr, D))
+    q.copy_(randn((100, H, D), 41))
+    k[-300:], v[-300:] = randn((300, Gr, D), 42), randn((300, Gr, D), 43)
+    packed(native, q, k, v, q_at, out, kv_at)
+    near = [c - (rows - 300) for c in kv_at]
+    want, tol = packed_oracle(f64(q), f64(k[-300:]), f64(v[-300:]), q_at, near, D ** -0.5, U[torch.float16])
+    check_close(f64(out), want, tol, "far rows")
+
+
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 32), (128, 4)])
+def test_pages_behind_four_gigabytes(native, D, bs):
+    drafts, H, Gr, pages = 6, 4, 2, (5 << 30) // (2 * bs * D * 2)
+    t = list(make_tree(2, drafts, H, Gr, D, bs, [130, 5], [6, 4], seed=44))
+    want, tol = tree_oracle(*t, D ** -0.5)
+    n = t[1].shape[0]
+    pools = torch.empty((2, pages, Gr, bs, D), dtype=torch.float16, device="cuda")
+    for i in range(2):
+        pools[i, -n:] = torch.tensor(t[1 + i]).cuda()
+    tables = i32(t[3] + (pages - n))
+    q, ctx, counts, parents = torch.tensor(t[0]).cuda(), i32(t[4]), i32(t[5]), i32(t[6])
+    out, status = torch.full(t[0].shape, 77.0, dtype=torch.float16, device="cuda"), i32([0])
+    ws = room(ops.tree_attention_workspace(native, q, pools[0], tables))
+    ops.tree_attention(native, q, pools[0], pools[1], tables, ctx, counts, parents, out, workspace=ws, status=status, stream=stream())
+    before = pools[:, -n:].clone()
+    path = i32([[0, 2, 5, 0, 0, 0], [1, 3, 0, 0, 0, 0]])
+    ops.cache_keep(native, pools[None, 0], pools[None, 1], tables, ctx, path, i32([3, 2]), status=status, stream=stream())
+    torch.cuda.synchronize()
+    check_close(f64(out), want, tol, "far pages")
+    for s, keep in enumerate(([0, 2, 5], [1, 3])):
+        src = [before[:, t[3][s, (t[4][s] + p) // bs], :, (t[4][s] + p) % bs].clone() for p in keep]
+        for j, r in enumerate(src):
+            to = t[4][s] + j
+            before[:, t[3][s, to // bs], :, to % bs] = r
+    assert torch.equal(pools[:, -n:].view(torch.int16), before.view(torch.int16)) and status.item() == 0
+
+
+def test_logits_behind_four_gigabytes(native):
+    wide = torch.empty((130, 1 << 24), device="cuda")      # 64 MB apart
+    x = wide[:, 5:1005]
+    x.copy_(randn((130, 1000), 45, torch.float32))
+    tok = np.arange(130, dtype=np.int32) * 7
+    check_logprobs(logprobs(native, x, i32(tok), 3), logprobs_oracle(f64(x), tok, 3), f64(x))
+
+
+def test_two_streams_at_once(native):
+    """Calls of two streams with a workspace each, long and short ones by turns, give what they give alone."""
+    H, Gr, D = 8, 2, 64
+    a, b = [300, 5, 700], [1, 2, 150]
+    q, k, v = randn((1005, H, D), 51), randn((1005, Gr, D), 52), randn((1005, Gr, D), 53)
+    t = [torch.tensor(x).cuda() for x in make_tree(5, 16, H, Gr, 128, 16, [2000, 3, 900, 0, 64], [16, 1, 9, 16, 0], seed=54)]
+    alone = [torch.full_like(q, 77.0), torch.full_like(q, 77.0), torch.full_like(t[0], 77.0)]
+    packed(native, q, k, v, offsets(a), alone[0])
+    packed(native, q, k, v, offsets(b), alone[1])
+    ws = [room(ops.packed_attention_workspace(native, q, k, 3)), room(ops.tree_attention_workspace(native, t[0], t[1], t[3]))]
+    ops.tree_attention(native, *t, alone[2], workspace=ws[1], stream=stream())
+    at = [i32(offsets(a)), i32(offsets(b))]
+    together = [[torch.full_like(x, 55.0) for x in alone] for _ in range(20)]
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for o in together:
+        ops.packed_attention(native, q, k, v, at[0], o[0], workspace=ws[0], stream=one)
+        ops.tree_attention(native, *t, o[2], workspace=ws[1], stream=two)
+        ops.packed_attention(native, q, k, v, at[1], o[1], workspace=ws[0], stream=one)
+    torch.cuda.synchronize()
+    for o in together:
+        assert torch.equal(o[0], alone[0]) and torch.equal(o[2], alone[2])
+        assert torch.equal(o[1][:153], alone[1][:153]) and (o[1][153:] == 55).all()
