@@ -52,11 +52,16 @@ def _code(dtype) -> int:
 
 
 def _view(native, x, name: str, types, ndim: int):
-    """(address, ggml type, shape, strides in elements, whether it is known to be dense) of an array of one of `types` with `ndim` dimensions on the
+    """(address, ggml type, shape, strides in elements or None where they are dense, dense) of an array of one of `types` with `ndim` dimensions on the
     handle's device."""
-    dense = False
+    try:        # a torch tensor whose type has been seen
+        code, shape, dense = _dtypes[x.dtype], x.shape, x.is_contiguous()
+        if code in types and len(shape) == ndim and x.get_device() == native.ordinal:
+            return x.data_ptr(), code, shape, None if dense else x.stride(), dense
+    except (AttributeError, KeyError):
+        pass
     if hasattr(x, "data_ptr"):
-        code, shape, strides, ptr, dense = _dtypes.get(x.dtype) or _code(x.dtype), x.shape, x.stride(), x.data_ptr(), x.is_contiguous()
+        code, shape, strides, ptr = _code(x.dtype), x.shape, x.stride(), x.data_ptr()
         if x.get_device() != native.ordinal:
             _invalid("%s lies on another device than the handle's (GPU %d)" % (name, native.ordinal))
     else:
@@ -65,26 +70,23 @@ def _view(native, x, name: str, types, ndim: int):
             _invalid("%s is not an array in device memory" % name)
         code, shape, ptr, strides = _code(face["typestr"]), face["shape"], face["data"][0], face.get("strides")
         size = _SIZE.get(code, 1)
-        if strides is None:
-            strides, n = [0] * len(shape), 1
-            for i in range(len(shape) - 1, -1, -1):
-                strides[i] = n
-                n *= shape[i]
-        elif any(b % size for b in strides):
-            _invalid("%s has strides that are no whole elements" % name)
-        else:
+        if strides is not None:
+            if any(b % size for b in strides):
+                _invalid("%s has strides that are no whole elements" % name)
             strides = [b // size for b in strides]
     if code not in types:
         _invalid("%s must be %s" % (name, " or ".join(_NAMES[t] for t in types)))
     if len(shape) != ndim:
         _invalid("%s must have %d dimensions, got %d" % (name, ndim, len(shape)))
-    return ptr, code, shape, strides, dense
+    return ptr, code, shape, strides, strides is None
 
 
 def _dense(view, name: str, first: int = 0) -> None:
     """Dimensions from `first` on are dense."""
-    _, _, shape, strides, dense = view
-    if dense or 0 in shape:
+    if view[4]:
+        return
+    _, _, shape, strides, _ = view
+    if 0 in shape:
         return
     n = 1
     for i in range(len(shape) - 1, first - 1, -1):
@@ -98,9 +100,9 @@ def _array(native, x, name: str, code: int, shape: tuple) -> int:
     if x is None:
         return 0
     try:
-        if x.shape == shape and _dtypes.get(x.dtype) == code and x.is_contiguous() and x.get_device() == native.ordinal:
+        if x.shape == shape and _dtypes[x.dtype] == code and x.is_contiguous() and x.get_device() == native.ordinal:
             return x.data_ptr()
-    except AttributeError:
+    except (AttributeError, KeyError):
         pass
     v = _view(native, x, name, (code,), len(shape))
     if tuple(v[2]) != shape:
@@ -115,15 +117,9 @@ def _given(x, name: str):
     return x
 
 
-def _step(view) -> int:
-    """Bytes from row to row; those of a dense row where there are not two."""
-    _, code, shape, strides, _ = view
-    if shape[0] > 1:
-        return strides[0] * _SIZE[code]
-    n = _SIZE[code]
-    for d in shape[1:]:
-        n *= d
-    return n
+def _step(view, row: int) -> int:
+    """Bytes from row to row, for rows of `row` bytes."""
+    return row if view[4] or view[2][0] < 2 else view[3][0] * _SIZE[view[1]]
 
 
 def _room(native, workspace) -> tuple:
@@ -166,6 +162,7 @@ def _packed_args(native, q, k, seqs, scale, v=None, out=None, q_offsets=0, kv_of
     if K[1] != Q[1]:
         _invalid("k must have the type of q")
     (rows, heads, size), (kv_rows, kv_heads, kv_size) = Q[2], K[2]
+    row, kv_row = heads * size * 2, kv_heads * size * 2
     if V[2] != K[2] or O[2] != Q[2] or kv_size != size:
         _invalid("q and out are [rows, heads, head size], k and v [rows, kv heads, head size]")
     _dense(Q, "q", 1)
@@ -174,7 +171,7 @@ def _packed_args(native, q, k, seqs, scale, v=None, out=None, q_offsets=0, kv_of
     _dense(O, "out", 1)
     room, room_bytes = _room(native, workspace)
     return _pack(_PACKED, Q[1], seqs, heads, kv_heads, size, 1.0 / math.sqrt(max(size, 1)) if scale is None else scale, rows, kv_rows, Q[0], K[0], V[0], O[0],
-                        _step(Q), _step(K), _step(V), _step(O), q_offsets, kv_offsets, room, room_bytes, _array(native, status, "status", I32, (1,)))
+                        _step(Q, row), _step(K, kv_row), _step(V, kv_row), _step(O, row), q_offsets, kv_offsets, room, room_bytes, _array(native, status, "status", I32, (1,)))
 
 
 def packed_attention_workspace(native, q, k, seqs: int) -> int:
@@ -248,7 +245,8 @@ def cache_keep(native, k_pools, v_pools, tables, context, path, counts, *, statu
     _dense(V, "v_pools", 1)
     _dense(T, "tables")
     _dense(P, "path")
-    a = _pack(_KEEP, layers, n, drafts, kv_heads, size, block_size, T[2][1], pages, K[0], V[0], _step(K), _step(V), T[0],
+    pool = pages * kv_heads * block_size * size * 2
+    a = _pack(_KEEP, layers, n, drafts, kv_heads, size, block_size, T[2][1], pages, K[0], V[0], _step(K, pool), _step(V, pool), T[0],
                    _array(native, _given(context, "context"), "context", I32, (n,)), _array(native, _given(counts, "counts"), "counts", I32, (n,)), P[0],
                    _array(native, status, "status", I32, (1,)))
     check(native.L.tlb_cache_keep(native.dev, a, _stream(stream)))
@@ -277,7 +275,7 @@ def token_logprobs(native, logits, tokens, logprob, entropy=None, top_ids=None, 
             _invalid("top_ids must have a row for each row of the logits")
         top = I[2][1]
     room, room_bytes = _room(native, workspace)
-    a = _pack(_SCORES, L[1], top, rows, vocab, L[0], _step(L), _array(native, tokens, "tokens", I32, (rows,)), _array(native, logprob, "logprob", F32, (rows,)),
+    a = _pack(_SCORES, L[1], top, rows, vocab, L[0], _step(L, vocab * _SIZE[L[1]]), _array(native, tokens, "tokens", I32, (rows,)), _array(native, logprob, "logprob", F32, (rows,)),
                      _array(native, entropy, "entropy", F32, (rows,)), _array(native, top_ids, "top_ids", I32, (rows, top)),
                      _array(native, top_logprobs, "top_logprobs", F32, (rows, top)), room, room_bytes, _array(native, status, "status", I32, (1,)))
     check(native.L.tlb_token_logprobs(native.dev, a, _stream(stream)))
