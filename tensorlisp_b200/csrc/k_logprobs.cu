@@ -220,10 +220,11 @@ __device__ __forceinline__ Key key_of(float x, uint32_t id) { return x > -CUDART
 __device__ __forceinline__ uint32_t id_of(Key k) { return 0xffffffffu - (uint32_t)k; }
 __device__ __forceinline__ float value_of(Key k) { return unorder((int)((uint32_t)(k >> 32) ^ 0x80000000u)); }
 
-// The k largest of n candidates at(i) to out[0..k) (0 where they run out). The k-th best of what groups of four threads have is a bound: what is at
-// least as good lies in k groups, which look through their shares again and put it on a list, whose entries then count who is in front of them.
+// The k largest of the threads' candidates, each(f) calls f for a thread's, to out[0..k) (0 where they run out). The k-th best of what groups of four
+// threads have is a bound: what is at least as good lies in k groups, which look through their shares again and put it on a list, whose entries then
+// count who is in front of them.
 // (Rounds of one maximum each took 24 us for 20 of 1000 segments and 20 of 2560 values; ranks of all 256 threads' bests 18.) The list holds LIST
-// entries: n up to LIST / (4 k) x THREADS; more candidates are picked in rounds.
+// entries: up to LIST / (4 k) of a thread; more candidates are picked in rounds.
 constexpr int GROUP = 4, GROUPS = THREADS / GROUP, LIST = 4096;
 static_assert(GROUPS >= LOGPROBS_MAX_TOP, "the bound is one group's");
 struct Select {
@@ -232,10 +233,9 @@ struct Select {
 };
 __device__ __forceinline__ bool select_takes(int64_t n, int k) { return (n + THREADS - 1) / THREADS * GROUP * k <= LIST; }
 template <typename F>
-__device__ __forceinline__ void select(int n, int k, const F &at, Key *out, Select &sh) {
+__device__ __forceinline__ void select(int k, const F &each, Key *out, Select &sh) {
     Key mine = 0;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += THREADS) mine = max(mine, at(i));
+    each([&](Key c) { mine = max(mine, c); });
     Key group = max(mine, (Key)__shfl_xor_sync(0xffffffffu, mine, 1));
     group = max(group, (Key)__shfl_xor_sync(0xffffffffu, group, 2));
     if (threadIdx.x % GROUP == 0) sh.best[threadIdx.x / GROUP] = group;
@@ -254,13 +254,10 @@ __device__ __forceinline__ void select(int n, int k, const F &at, Key *out, Sele
     }
     __syncthreads();
     const Key bound = sh.bound;
-    if (mine >= bound) {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += THREADS) {
-            const Key c = at(i);
+    if (mine >= bound)
+        each([&](Key c) {
             if (c >= bound) sh.list[atomicAdd(&sh.n, 1)] = c;
-        }
-    }
+        });
     __syncthreads();
     const int listed = sh.n;
     for (int i = threadIdx.x; i < listed; i += THREADS) {
@@ -318,6 +315,8 @@ __global__ void __launch_bounds__(lp::THREADS) k_logprobs_finish(const __grid_co
     const Logprobs &a = p.a;
     const T *row = reinterpret_cast<const T *>((const char *)a.logits + row_i * a.stride);
     if (threadIdx.x < 32) {   // the other warps begin to look for the alternatives
+        const int32_t tok = a.logprob && a.tokens ? a.tokens[row_i] : -1;
+        const float logit = tok >= 0 && tok < a.vocab ? value(row[tok]) : 0.f;
         Sums v = {-CUDART_INF_F, 0.f, 0.f};
         for (int i = threadIdx.x; i < p.splits; i += 32) {
             Sums w = p.part[row_i * p.splits + i];
@@ -334,10 +333,9 @@ __global__ void __launch_bounds__(lp::THREADS) k_logprobs_finish(const __grid_co
             row_s = v;
             log_s_s = log_s;
             if (a.logprob) {
-                const int32_t tok = a.tokens ? a.tokens[row_i] : -1;
                 float y = 0.f;
                 if (tok >= 0 && tok < a.vocab) {
-                    y = undefined ? CUDART_NAN_F : (empty ? -CUDART_INF_F : (value(row[tok]) - v.m) - log_s);
+                    y = undefined ? CUDART_NAN_F : (empty ? -CUDART_INF_F : (logit - v.m) - log_s);
                 } else if (tok != -1) {
                     y = CUDART_NAN_F;
                     if (a.err) report_error(a.err, TLB_ERR_INDEX);
@@ -351,13 +349,39 @@ __global__ void __launch_bounds__(lp::THREADS) k_logprobs_finish(const __grid_co
     const float *seg_max = p.seg_max + row_i * p.turns * UNROLL;
     const int shift = shift_of(row), n = p.turns * UNROLL;
     const auto segment = [&](int i) { return key_of(seg_max[i], (uint32_t)i); };
-    if (select_takes(n, a.top)) select(n, a.top, segment, segs, sel);
-    else pick(n, a.top, segment, segs, rounds);
-    static_assert(LOGPROBS_MAX_TOP * 256 / THREADS * GROUP * LOGPROBS_MAX_TOP <= LIST, "the values of the segments always fit the list");
-    select(a.top * SEG, a.top, [&](int i) -> Key {
-        const Key seg = segs[i / SEG];
-        const int64_t id = (int64_t)id_of(seg) * SEG + i % SEG - shift;
-        return seg && id >= 0 && id < a.vocab ? key_of(value(row[id]), (uint32_t)id) : 0;
+    if (select_takes(n, a.top)) {
+        Key near[4];   // one trip for the first of a thread's
+#pragma unroll
+        for (int u = 0; u < 4; u++) near[u] = threadIdx.x + u * THREADS < n ? segment(threadIdx.x + u * THREADS) : 0;
+        select(a.top, [&](const auto &f) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) f(near[u]);
+#pragma unroll 4
+            for (int i = threadIdx.x + 4 * THREADS; i < n; i += THREADS) f(segment(i));
+        }, segs, sel);
+    } else {
+        pick(n, a.top, segment, segs, rounds);
+    }
+    // A warp's segments, in 16-byte pieces that stay in registers
+    constexpr int N = Vec<T>::N, MOST = LOGPROBS_MAX_TOP / WARPS;
+    static_assert(MOST * N * GROUP * LOGPROBS_MAX_TOP <= LIST, "the values of the segments always fit the list");
+    uint4 raw[MOST];
+    int first[MOST];
+#pragma unroll
+    for (int u = 0; u < MOST; u++) {
+        const int i = (threadIdx.x >> 5) + u * WARPS;
+        const Key seg = i < a.top ? segs[i] : 0;
+        first[u] = seg ? (int)id_of(seg) * SEG - shift + (threadIdx.x & 31) * N : (int)a.vocab;
+        if (seg) raw[u] = load_piece<T>(row, (int)a.vocab, first[u]);
+    }
+    select(a.top, [&](const auto &f) {
+#pragma unroll
+        for (int u = 0; u < MOST; u++) {
+            if (first[u] >= (int)a.vocab) continue;
+            const T *e = reinterpret_cast<const T *>(&raw[u]);
+#pragma unroll
+            for (int i = 0; i < N; i++) f(key_of(value(e[i]), (uint32_t)(first[u] + i)));   // past the ends: -inf
+        }
     }, best, sel);
     if (threadIdx.x < a.top) {
         const Sums v = row_s;
