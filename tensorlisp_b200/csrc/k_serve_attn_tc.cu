@@ -71,6 +71,13 @@ struct Place {
     int seq, kvh, r;
     int64_t off;    // units of this row tile in front of the place
 };
+// The row tile that a CTA's stretch ends in, if it begins there and others go on with it
+struct Cut {
+    int parts;      // 0: none
+    int kvh, token0;
+    int q0, nq;     // the sequence's queries
+    int pad[3];
+};
 struct Params {
     CUtensorMap q, k, v;
     ServeAttn a;
@@ -78,7 +85,7 @@ struct Params {
     int pool_rows;            // paged: rows of a pool
     int group, tpt, tt;       // heads per KV head; tokens of a row tile; of the row tiles that a unit covers
     int ctas, overhead, min_units;   // of a row tile; a CTA's least share
-    Place *ends;              // [CTA]: where its stretch ends, which tells k_serve_join what it cuts
+    Cut *cuts;                // [CTA], for k_serve_join
     float *partial;           // [CTA][2]: (m, l) of the rows, then O as [hsp / 4][rows][4], which the writers' lanes (rows) fill side by side
 };
 
@@ -544,11 +551,13 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
         // ---- copies. The keys of a segment's first tiles are on their way before its queries, whose room the segment in front still uses.
         Walk<PAGED, KT> walk;
+        int64_t share, stretch;
         {
             LaneSeq seq0;
-            const int64_t total = total_units<PAGED, KT>(p, seq0), share = share_of(p, total), first = share * blockIdx.x;
-            if (lane == 0 && blockIdx.x == 0) p.ends[p.ctas].off = share;
-            walk.left = min(share, total - first);
+            const int64_t total = total_units<PAGED, KT>(p, seq0);
+            share = share_of(p, total);
+            const int64_t first = share * blockIdx.x;
+            walk.left = stretch = min(share, total - first);
             walk.at = {p.a.seqs, 0, 0, 0};
             if (walk.left > 0) {
                 walk.at = find_unit<PAGED, KT>(p, first, seq0, walk.sq);
@@ -600,7 +609,15 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             __syncwarp();
             seg++;
         }
-        if (lane == 0) p.ends[blockIdx.x] = walk.left == 0 ? walk.at : Place{p.a.seqs, 0, 0, 0};
+        if (lane == 0) {
+            Cut cut{};
+            const int64_t off = walk.at.off;
+            if (walk.left == 0 && off > 0 && off <= stretch) {   // further than the stretch is long: it begins in one in front
+                const int n = key_tiles<PAGED, KT>(p, walk.sq, walk.at.r);
+                if (off < n) cut = {1 + (int)divide(n - off + share - 1, share), walk.at.kvh, walk.at.r * p.tt, (int)walk.sq.q0, walk.sq.nq, {}};
+            }
+            p.cuts[blockIdx.x] = cut;
+        }
     } else if (warp == 1) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
         // ---- MMA issue: S of a tile follows O of the tile that had its columns, which has read the P that it overwrites. With SHARE streams are constants of the
@@ -928,57 +945,61 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     if (tid == 0 && s_fail && p.a.err) report_error(p.a.err, 2);
 }
 
-// Row tiles that were cut (3 to 9 us beside the launch in front, whose plan it reads): CTA (c, rows) adds up the parts of the one that begins in stretch c of the line and reaches over its end.
+// Row tiles that were cut: CTA (c, rows) adds up the parts of the one that begins in stretch c of the line and reaches over its end. Bound by two trips to L2, what
+// is cut and then all of (m, l, O) of up to four parts at once, and by the launch.
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
-__global__ void __launch_bounds__(128) k_serve_join(const __grid_constant__ sat::Params p) {
+__global__ void __launch_bounds__(256) k_serve_join(const __grid_constant__ sat::Params p) {
     using namespace sat;
-    constexpr int NQ = SHARE ? 2 : 1, ROWS = NQ * T, SLOT = ROWS * (2 + HSP);
+    constexpr int NQ = SHARE ? 2 : 1, ROWS = NQ * T, SLOT = ROWS * (2 + HSP), W = HSP / 32;   // float4s of a thread
     griddep_launch();
     griddep_wait();
     const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Place w = p.ends[c];
-    if (w.seq >= p.a.seqs || w.off == 0) return;   // nothing is cut here
-    const Place v = c ? p.ends[c - 1] : Place{0, 0, 0, 0};
-    if (v.off > 0 && v.seq == w.seq && v.kvh == w.kvh && v.r == w.r) return;   // it begins in a stretch in front
-    const ServeSeq sq = serve_seq(p.a, w.seq);
-    const int n = key_tiles<PAGED, key_tile(HSP, SHARE)>(p, sq, w.r);
-    if (w.off >= n) return;   // all of its key tiles lie in this stretch
-    const int parts = 1 + (int)((n - w.off + p.ends[p.ctas].off - 1) / p.ends[p.ctas].off);
-    // 32 rows: a lane's row is its own, a warp's columns a quarter of them
+    const Cut cut = p.cuts[c];
+    // 32 rows: a lane's row is its own, a warp's columns an eighth of them
     const int row = blockIdx.y * 32 + lane, x = row / T, rr = row % T;
-    const int token = w.r * p.tt + x * p.tpt + rr / p.group, head = w.kvh * p.group + rr % p.group;
-    if (rr >= p.tpt * p.group || token >= (PAGED ? p.a.drafts : sq.nq)) return;
+    const int token = cut.token0 + x * p.tpt + rr / p.group, head = cut.kvh * p.group + rr % p.group;
+    if (cut.parts == 0 || rr >= p.tpt * p.group || token >= (PAGED ? p.a.drafts : cut.nq)) return;
     auto slot = [&](int i) { return p.partial + ((size_t)(c + i) * 2 + (i ? 0 : 1)) * SLOT; };
-    float m = -CUDART_INF_F;
-#pragma unroll 4
-    for (int i = 0; i < parts; i++) {
-        const float2 ml = *reinterpret_cast<const float2 *>(slot(i) + row * 2);
-        m = fmaxf(m, ml.y == 0.f ? -CUDART_INF_F : ml.x);   // l = 0: the row sees nothing in this part
-    }
-    if (m == -CUDART_INF_F) m = 0.f;
-    float l = 0.f;
-    float4 o[HSP / 16];
+    float m = -CUDART_INF_F, l = 0.f;
+    float4 o[W];
 #pragma unroll
-    for (int e = 0; e < HSP / 16; e++) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-    for (int i = 0; i < parts; i++) {
-        const float2 ml = *reinterpret_cast<const float2 *>(slot(i) + row * 2);
-        const float4 *s = reinterpret_cast<const float4 *>(slot(i) + ROWS * 2) + (size_t)(warp * (HSP / 16)) * ROWS + row;
-        float4 y[HSP / 16];
+    for (int e = 0; e < W; e++) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < cut.parts; i0 += 4) {
+        float2 ml[4];
+        float4 y[4][W];
 #pragma unroll
-        for (int e = 0; e < HSP / 16; e++) y[e] = s[(size_t)e * ROWS];
-        if (ml.y != 0.f) {
-            const float f = ex2(ml.x - m);
-            l = fmaf(ml.y, f, l);
+        for (int u = 0; u < 4; u++) {
+            ml[u] = make_float2(0.f, 0.f);
+            if (i0 + u >= cut.parts) continue;
+            ml[u] = *reinterpret_cast<const float2 *>(slot(i0 + u) + row * 2);
+            const float4 *s = reinterpret_cast<const float4 *>(slot(i0 + u) + ROWS * 2) + (size_t)(warp * W) * ROWS + row;
 #pragma unroll
-            for (int e = 0; e < HSP / 16; e++) o[e] = make_float4(fmaf(y[e].x, f, o[e].x), fmaf(y[e].y, f, o[e].y), fmaf(y[e].z, f, o[e].z), fmaf(y[e].w, f, o[e].w));
+            for (int e = 0; e < W; e++) y[u][e] = s[(size_t)e * ROWS];
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (ml[u].y != 0.f) top = fmaxf(top, ml[u].x);   // l = 0: the row sees nothing in this part
+        if (top == -CUDART_INF_F) continue;
+        const float keep = ex2(m - top);
+        m = top;
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < W; e++) o[e] = make_float4(o[e].x * keep, o[e].y * keep, o[e].z * keep, o[e].w * keep);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (ml[u].y == 0.f) continue;
+            const float f = ex2(ml[u].x - m);
+            l = fmaf(ml[u].y, f, l);
+#pragma unroll
+            for (int e = 0; e < W; e++) o[e] = make_float4(fmaf(y[u][e].x, f, o[e].x), fmaf(y[u][e].y, f, o[e].y), fmaf(y[u][e].z, f, o[e].z), fmaf(y[u][e].w, f, o[e].w));
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    char *dst = (char *)p.a.out + (sq.q0 + token) * p.a.out_stride + (int64_t)head * p.a.hs * 2;
+    char *dst = (char *)p.a.out + (int64_t)(cut.q0 + token) * p.a.out_stride + (int64_t)head * p.a.hs * 2;
 #pragma unroll
-    for (int e = 0; e < HSP / 16; e += 2) {
-        const int col = warp * (HSP / 4) + e * 4;
+    for (int e = 0; e < W; e += 2) {
+        const int col = warp * (HSP / 8) + e * 4;
         if (col < p.a.hs)
             *reinterpret_cast<uint4 *>(dst + col * 2) = make_uint4(round2<BF16>(o[e].x * inv, o[e].y * inv), round2<BF16>(o[e].z * inv, o[e].w * inv),
                                                                    round2<BF16>(o[e + 1].x * inv, o[e + 1].y * inv), round2<BF16>(o[e + 1].z * inv, o[e + 1].w * inv));
@@ -1010,16 +1031,16 @@ static int sat_ctas(const ServeAttn &a, int sm_count) {
     const double units = (double)tiles * a.kv_heads * (double)(keys + sat::overhead(share)), least = 1 + sat::overhead(share);
     return units / least < sm_count ? std::max(1, (int)(units / least + 1)) : sm_count;
 }
-static uint64_t sat_ends_bytes(int ctas) { return ((uint64_t)(ctas + 1) * sizeof(sat::Place) + 255) / 256 * 256; }   // the last one: the size of a share
+static uint64_t sat_cuts_bytes(int ctas) { return ((uint64_t)ctas * sizeof(sat::Cut) + 255) / 256 * 256; }
 uint64_t serve_attn_tc_scratch_bytes(const ServeAttn &a, int sm_count) {
     const uint64_t ctas = (uint64_t)sat_ctas(a, sm_count);
-    return sat_ends_bytes((int)ctas) + ctas * 2 * (sat_share(a, sm_count) ? 2 : 1) * sat::T * (2 + sat_padded(a)) * 4;
+    return sat_cuts_bytes((int)ctas) + ctas * 2 * (sat_share(a, sm_count) ? 2 : 1) * sat::T * (2 + sat_padded(a)) * 4;
 }
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
 static cudaError_t sat_launch(const sat::Params &p, int ctas, cudaStream_t st) {
     cudaError_t e = launch_pdl(k_serve_attn_tc<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas), dim3(sat::THREADS), sat::smem_bytes(HSP, SHARE), st, p);
     if (e == cudaSuccess && ctas > 1 && most_key_tiles(p.a, sat::key_tile(HSP, SHARE)) > 1)   // a single key tile is never cut
-        e = launch_pdl(k_serve_join<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas - 1, (SHARE ? 2 : 1) * sat::T / 32), dim3(128), 0, st, p);
+        e = launch_pdl(k_serve_join<HSP, BF16, PAGED, SHARE>, dim3((unsigned)ctas - 1, (SHARE ? 2 : 1) * sat::T / 32), dim3(256), 0, st, p);
     return e;
 }
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
@@ -1074,8 +1095,8 @@ cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count
     }
     if (e != cudaSuccess) return e;
     const int ctas = p.ctas = sat_ctas(a, sm_count);
-    p.ends = (Place *)scratch;
-    p.partial = (float *)((char *)scratch + sat_ends_bytes(ctas));
+    p.cuts = (Cut *)scratch;
+    p.partial = (float *)((char *)scratch + sat_cuts_bytes(ctas));
     if (a.paged) return a.hs <= 64 ? sat_launch<64, false, true, false>(p, ctas, st) : sat_launch<128, false, true, false>(p, ctas, st);
     if (a.hs <= 64) {
         if (a.bf16) return share ? sat_launch<64, true, false, true>(p, ctas, st) : sat_launch<64, true, false, false>(p, ctas, st);
