@@ -61,9 +61,11 @@ __host__ __device__ constexpr int key_tile(int hsp, bool share) { return share &
 // multiplied: 24 prompts of up to 1000 tokens, 16 heads of 64, 62 us against 74 with one tile of 128 keys. Heads of 128 have room for two only of 64 keys: 1 x 8192
 // 531 us against 483
 __host__ __device__ constexpr int buffers(int hsp, bool share) { return share && hsp == 64 ? 2 : 1; }
-// What a row tile costs beside its key tiles, in key tiles, and with it a CTA's least share. us with 1, 2, 4, 6: 1 x 8192 546, 506, 500, 511; tree 48 x 32 over
+// What a row tile costs beside its key tiles, in key tiles. us with 1, 2, 4, 6: 1 x 8192 546, 506, 500, 511; tree 48 x 32 over
 // up to 8192 182, 180, 174, 172. With 2, 3, 5, 8: 24 x 1000 of head size 64 63, 60, 62, 66
 constexpr int overhead(bool share) { return share ? 3 : 5; }
+// A CTA's least share, in key tiles. us with 3, 4, 6 of 64: tree 1 x 8 behind 500 12.6, 13.4, 14.6; behind 2000 14.9, 15.5, 15.5; prompt of 37 behind 500 14.1, 14.3, 15.1
+constexpr int least_share(bool share) { return share ? 4 : 3; }
 __host__ __device__ constexpr int stages(int hsp, bool share) { return hsp == 128 ? (share ? 2 : 6) : 8; }
 __host__ __device__ constexpr int smem_bytes(int hsp, bool share) { return ((share ? 2 : 1) * T + 2 * stages(hsp, share) * key_tile(hsp, share)) * hsp * 2; }
 
@@ -1028,7 +1030,7 @@ static int sat_ctas(const ServeAttn &a, int sm_count) {
     const int64_t tt = (int64_t)(sat::T / (a.heads / a.kv_heads)) * (share ? 2 : 1);
     const int64_t tiles = a.paged ? (a.drafts + tt - 1) / tt * a.seqs : a.q_rows / tt + a.seqs;
     const int64_t kt = sat::key_tile(sat_padded(a), share), keys = most_key_tiles(a, (int)kt);
-    const double units = (double)tiles * a.kv_heads * (double)(keys + sat::overhead(share)), least = 1 + sat::overhead(share);
+    const double units = (double)tiles * a.kv_heads * (double)(keys + sat::overhead(share)), least = sat::least_share(share);
     return units / least < sm_count ? std::max(1, (int)(units / least + 1)) : sm_count;
 }
 static uint64_t sat_cuts_bytes(int ctas) { return ((uint64_t)ctas * sizeof(sat::Cut) + 255) / 256 * 256; }
@@ -1073,7 +1075,7 @@ cudaError_t launch_serve_attn_tc(const ServeAttn &a, void *scratch, int sm_count
     p.tt = p.tpt * (share ? 2 : 1);
     const int kt = key_tile(sat_padded(a), share);
     p.overhead = overhead(share);
-    p.min_units = 1 + p.overhead;
+    p.min_units = least_share(share);
     const uint64_t hs = (uint64_t)a.hs;
     cudaError_t e;
     {
