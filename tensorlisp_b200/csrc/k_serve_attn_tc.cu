@@ -25,7 +25,7 @@
 // What bounds it. Prompts: a 128 x 128 x 16 MMA takes 60 to 75 cycles to issue and execute, which is 62 % of the time of 1 x 8192 tokens (32 + 8 heads of 128: 480 us,
 // 1.15 PFLOP/s while the clock holds, 970 TFLOP/s under the power cap); the rest is the chain of a stream (read S 250 cycles, maximum 400, exponentials 1400, P V and the
 // next Q K 1024) where the other one does not cover it. Drafts: the keys' and values' bytes, pages of 4 KB in random order: 48 sequences x 32 drafts over up to 8192
-// tokens 166 us = 5.1 TB/s. Short calls: the plan (5000 cycles from the kernel's start to the first copy), an epilogue of 3000 and the joining launch.
+// tokens 157 to 169 us = 5.0 to 5.4 TB/s. Short calls: the plan (5000 cycles from the kernel's start to the first copy), an epilogue of 3000 and the joining launch (3 us).
 // Polynomials for some of the exponentials (25, 38, 50 %: 500 us -> 527, 555, 622), P handed over in halves (489 -> 500) and P beside S for heads of 64 (74 -> 82)
 // lost.
 //
