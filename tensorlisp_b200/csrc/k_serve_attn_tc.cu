@@ -465,7 +465,8 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     __shared__ float pair_ml[2][T][2];
     volatile int *fail = &s_fail;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // warp: known to be the same in all lanes, so that roles are branched to as one (with tid >> 5 alone: trees of 32 x 16 64 -> 71 us, 24 x 1000 63 -> 67)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
         mbar_init(&bar_q, 1);
         mbar_init(&bar_qfree, 1);
@@ -502,6 +503,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     if (warp == 2 && blockIdx.x == 0 && p.a.err) {
         for (int s = lane; s < p.a.seqs; s += 32)
             if (!serve_seq(p.a, s).ok) report_error(p.a.err, TLB_ERR_INDEX);
+        __syncwarp();
     }
     const uint32_t tmem = tmem_base_s;
     Segment g;
@@ -549,188 +551,187 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             behind(j);
         }
     };
-    if (warp == 0) {
+    if (warp < 4) {   // one instruction for the whole warpgroup, in front of its roles
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
-        // ---- copies. The keys of a segment's first tiles are on their way before its queries, whose room the segment in front still uses.
-        Walk<PAGED, KT> walk;
-        int64_t share, stretch;
-        {
-            LaneSeq seq0;
-            const int64_t total = total_units<PAGED, KT>(p, seq0);
-            share = share_of(p, total);
-            const int64_t first = share * blockIdx.x;
-            walk.left = stretch = min(share, total - first);
-            walk.at = {p.a.seqs, 0, 0, 0};
-            if (walk.left > 0) {
-                walk.at = find_unit<PAGED, KT>(p, first, seq0, walk.sq);
-                walk.tiles = row_tiles<PAGED>(p, walk.sq);
-                walk.loaded = walk.at.seq;
+        if (warp == 0) {
+            // ---- copies. The keys of a segment's first tiles are on their way before its queries, whose room the segment in front still uses.
+            Walk<PAGED, KT> walk;
+            int64_t share, stretch;
+            {
+                LaneSeq seq0;
+                const int64_t total = total_units<PAGED, KT>(p, seq0);
+                share = share_of(p, total);
+                const int64_t first = share * blockIdx.x;
+                walk.left = stretch = min(share, total - first);
+                walk.at = {p.a.seqs, 0, 0, 0};
+                if (walk.left > 0) {
+                    walk.at = find_unit<PAGED, KT>(p, first, seq0, walk.sq);
+                    walk.tiles = row_tiles<PAGED>(p, walk.sq);
+                    walk.loaded = walk.at.seq;
+                }
             }
-        }
-        auto tell = [&](const Segment &x) {
-            const int r = g_at % SEG_RING;
-            mbar_wait_nap(&bar_segfree[r], (uint32_t)(g_at / SEG_RING + 1) & 1u, fail, 32);
-            if (lane == 0) {
-                segs[r] = x;
-                mbar_arrive(&bar_seg[r]);
-            }
-            g_at++;
-        };
-        int tile = 0, seg = 0;
-        Segment ahead;
-        auto look_ahead = [&]() {
-            if (!walk.next(p, ahead)) ahead.t0 = -1;
-            tell(ahead);
-        };
-        look_ahead();
-        while (ahead.t0 >= 0 && !__any_sync(0xffffffffu, *fail)) {
-            g = ahead;
-            if (g.t1 == g.t0) {   // a row tile that sees nothing has no part in the pipeline's counts
-                look_ahead();
-                continue;
-            }
-            bool have_q = false;
-            auto load_q = [&]() {
+            auto tell = [&](const Segment &x) {
+                const int r = g_at % SEG_RING;
+                mbar_wait_nap(&bar_segfree[r], (uint32_t)(g_at / SEG_RING + 1) & 1u, fail, 32);
                 if (lane == 0) {
-                    mbar_wait_nap(&bar_qfree, (uint32_t)(seg + 1) & 1u, fail, 32);
-                    mbar_expect_tx(&bar_q, (uint32_t)(NQ * HALVES * 128 * p.group * p.tpt));
-                    for (int x = 0; x < NQ; x++)
-                        for (int h = 0; h < HALVES; h++)
-                            tma_3d(qs + x * QTILE + h * QHALF, &p.q, h * 64, g.kvh * p.group, g.q0 + g.token0 + x * p.tpt, &bar_q);
+                    segs[r] = x;
+                    mbar_arrive(&bar_seg[r]);
                 }
-                have_q = true;
+                g_at++;
             };
-            const int look_at = min(g.t0 + 1, g.t1 - 1);
-            copy_tiles(ks, &p.k, bar_k, bar_kfree, tile, [&](int j) {
-                if (!have_q && (j - g.t0 >= NS || __any_sync(0xffffffffu, mbar_test(su32(&bar_qfree), (uint32_t)(seg + 1) & 1u)))) load_q();
-            }, [&](int j) {
-                if (j == look_at) look_ahead();   // the next segment, while this one's tiles are on their way
-            });
-            if (__any_sync(0xffffffffu, *fail)) break;
-            if (!have_q) load_q();
-            __syncwarp();
-            seg++;
-        }
-        if (lane == 0) {
-            Cut cut{};
-            const int64_t off = walk.at.off;
-            if (walk.left == 0 && off > 0 && off <= stretch) {   // further than the stretch is long: it begins in one in front
-                const int n = key_tiles<PAGED, KT>(p, walk.sq, walk.at.r);
-                if (off < n) cut = {1 + (int)divide(n - off + share - 1, share), walk.at.kvh, walk.at.r * p.tt, (int)walk.sq.q0, walk.sq.nq, {}};
-            }
-            p.cuts[blockIdx.x] = cut;
-        }
-    } else if (warp == 1) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
-        // ---- MMA issue: S of a tile follows O of the tile that had its columns, which has read the P that it overwrites. With SHARE streams are constants of the
-        // code: with them taken from a step's number, 1 x 8192 takes 500 us against 483 and 24 x 1000 of head size 64 73 against 64.
-        const bool leader = elect_one();
-        int tile = 0, seg = 0;
-        uint32_t n_p[2] = {0, 0};
-        while (next()) {
-            const int n = g.t1 - g.t0;
-            if (n == 0) continue;
-            auto buffer = [&](int i) { return BUFS == 2 ? (tile + i) & 1 : 0; };
-            auto column = [&](int x, int i) { return (uint32_t)(x * T + buffer(i) * KT); };   // of S and P
-            auto issue_s = [&](int x, int i) {
-                const int s = (tile + i) % NS;
-                tc_fence_after();
-                if (leader) {
-#pragma unroll
-                    for (int h = 0; h < HALVES; h++) {
-                        const uint64_t qd = plain::desc_sw128(su32(qs + (SHARE ? x * QTILE : 0) + h * QHALF)), kd = plain::desc_sw128(su32(ks + s * TILE + h * KHALF));
-#pragma unroll
-                        for (int e = 0; e < 4; e++) umma_f16(tmem + column(x, i), qd + 2 * e, kd + 2 * e, IDESC_QK, (h | e) ? 1u : 0u);
+            int tile = 0, seg = 0;
+            Segment ahead;
+            auto look_ahead = [&]() {
+                if (!walk.next(p, ahead)) ahead.t0 = -1;
+                tell(ahead);
+            };
+            look_ahead();
+            while (ahead.t0 >= 0 && !__any_sync(0xffffffffu, *fail)) {
+                g = ahead;
+                if (g.t1 == g.t0) {   // a row tile that sees nothing has no part in the pipeline's counts
+                    look_ahead();
+                    continue;
+                }
+                bool have_q = false;
+                auto load_q = [&]() {
+                    if (lane == 0) {
+                        mbar_wait_nap(&bar_qfree, (uint32_t)(seg + 1) & 1u, fail, 32);
+                        mbar_expect_tx(&bar_q, (uint32_t)(NQ * HALVES * 128 * p.group * p.tpt));
+                        for (int x = 0; x < NQ; x++)
+                            for (int h = 0; h < HALVES; h++)
+                                tma_3d(qs + x * QTILE + h * QHALF, &p.q, h * 64, g.kvh * p.group, g.q0 + g.token0 + x * p.tpt, &bar_q);
                     }
-                    umma_commit(&bar_s[x][buffer(i)]);
-                    if (!SHARE || x == 1) {
-                        umma_commit(&bar_kfree[s]);
-                        if (i == n - 1) umma_commit(&bar_qfree);
-                    }
-                }
+                    have_q = true;
+                };
+                const int look_at = min(g.t0 + 1, g.t1 - 1);
+                copy_tiles(ks, &p.k, bar_k, bar_kfree, tile, [&](int j) {
+                    if (!have_q && (j - g.t0 >= NS || __any_sync(0xffffffffu, mbar_test(su32(&bar_qfree), (uint32_t)(seg + 1) & 1u)))) load_q();
+                }, [&](int j) {
+                    if (j == look_at) look_ahead();   // the next segment, while this one's tiles are on their way
+                });
+                if (__any_sync(0xffffffffu, *fail)) break;
+                if (!have_q) load_q();
                 __syncwarp();
-            };
-            auto issue_o = [&](int x, int i) {
-                const int s = (tile + i) % NS;
-                mbar_wait_nap(&bar_p[x][buffer(i)], (BUFS == 2 ? (uint32_t)(tile + i) >> 1 : n_p[x]) & 1u, fail, 0);
-                if (i == 0 && x == 0 && seg > 0) mbar_wait_nap(&bar_od, (uint32_t)(seg - 1) & 1u, fail, 0);
-                tc_fence_after();
-                if (leader) {
-                    const uint64_t vd = desc_mn<KHALF>(su32(vs + s * TILE));
-#pragma unroll
-                    for (int e = 0; e < KT / 16; e++)
-                        umma_f16_ta(tmem + O_COL + (uint32_t)(x * T), tmem + column(x, i) + (uint32_t)(e * 8), vd + (uint64_t)(e * 128), IDESC_PV, (i > (SHARE ? 0 : 1) || e) ? 1u : 0u);
-                    umma_commit(&bar_o[x][buffer(i)]);
-                    if (!SHARE || x == 1) umma_commit(&bar_vfree[s]);
-                }
-                __syncwarp();
-                n_p[x]++;
-            };
-            auto wait_for = [&](uint64_t *bar, int i) { mbar_wait_nap(&bar[(tile + i) % NS], (uint32_t)((tile + i) / NS) & 1u, fail, 0); };
-            mbar_wait_nap(&bar_q, (uint32_t)seg & 1u, fail, 0);
-            // (taking a P that is ready before keys that are not, so that a tile of values is free sooner: 185 us against 177 at 48 x 4096)
-            constexpr int AHEAD = SHARE ? BUFS : 2;
-            for (int i = 0; i < min(AHEAD, n); i++) {
-                wait_for(bar_k, i);
-                issue_s(SHARE ? 0 : i, i);
-                if (SHARE) issue_s(1, i);
+                seg++;
             }
-            for (int i = 0; i < n; i++) {
-                const bool more = i + AHEAD < n;
-                wait_for(bar_fix, i);
-                issue_o(SHARE ? 0 : i & 1, i);
-                if (more) {
-                    wait_for(bar_k, i + AHEAD);
-                    issue_s(SHARE ? 0 : i & 1, i + AHEAD);
+            if (lane == 0) {
+                Cut cut{};
+                const int64_t off = walk.at.off;
+                if (walk.left == 0 && off > 0 && off <= stretch) {   // further than the stretch is long: it begins in one in front
+                    const int n = key_tiles<PAGED, KT>(p, walk.sq, walk.at.r);
+                    if (off < n) cut = {1 + (int)divide(n - off + share - 1, share), walk.at.kvh, walk.at.r * p.tt, (int)walk.sq.q0, walk.sq.nq, {}};
                 }
-                if (SHARE) {
-                    issue_o(1, i);
-                    if (more) issue_s(1, i + AHEAD);
-                }
+                p.cuts[blockIdx.x] = cut;
             }
-            tile += n;
-            seg++;
-        }
-    } else if (warp == 2) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
-        // ---- every tile of values passes here, in order, on its way to the MMAs. Special ones: rows behind the end become zero, the others are
-        // looked through
-        int tile = 0, seg = 0;
-        while (next()) {
-            if (g.t1 == g.t0) continue;
-            for (int j = g.t0; j < g.t1; j++, tile++) {
-                const int s = tile % NS;
-                mbar_wait_nap(&bar_v[s], (uint32_t)(tile / NS) & 1u, fail, 0);
-                if (j >= g.special) {
-                    const int live = min(KT, g.nk - j * KT);
-                    uint4 *v = reinterpret_cast<uint4 *>(vs + s * TILE);
-                    constexpr uint32_t EXP = BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = BF16 ? 0x00800080u : 0x04000400u;   // one more than all ones carries into the sign
-                    uint32_t odd = 0;
-#pragma unroll 8
-                    for (int i = lane; i < TILE / 16; i += 32) {
-                        if (((i >> 3) & (KT - 1)) >= live) {
-                            v[i] = make_uint4(0, 0, 0, 0);
-                        } else {
-                            const uint4 w = v[i];
-                            odd |= ((w.x & EXP) + ONE) | ((w.y & EXP) + ONE) | ((w.z & EXP) + ONE) | ((w.w & EXP) + ONE);
+        } else if (warp == 1) {
+            // ---- MMA issue: S of a tile follows O of the tile that had its columns, which has read the P that it overwrites. With SHARE streams are constants of the
+            // code: with them taken from a step's number, 1 x 8192 takes 500 us against 483 and 24 x 1000 of head size 64 73 against 64.
+            const bool leader = elect_one();
+            int tile = 0, seg = 0;
+            uint32_t n_p[2] = {0, 0};
+            while (next()) {
+                const int n = g.t1 - g.t0;
+                if (n == 0) continue;
+                auto buffer = [&](int i) { return BUFS == 2 ? (tile + i) & 1 : 0; };
+                auto column = [&](int x, int i) { return (uint32_t)(x * T + buffer(i) * KT); };   // of S and P
+                auto issue_s = [&](int x, int i) {
+                    const int s = (tile + i) % NS;
+                    tc_fence_after();
+                    if (leader) {
+    #pragma unroll
+                        for (int h = 0; h < HALVES; h++) {
+                            const uint64_t qd = plain::desc_sw128(su32(qs + (SHARE ? x * QTILE : 0) + h * QHALF)), kd = plain::desc_sw128(su32(ks + s * TILE + h * KHALF));
+    #pragma unroll
+                            for (int e = 0; e < 4; e++) umma_f16(tmem + column(x, i), qd + 2 * e, kd + 2 * e, IDESC_QK, (h | e) ? 1u : 0u);
+                        }
+                        umma_commit(&bar_s[x][buffer(i)]);
+                        if (!SHARE || x == 1) {
+                            umma_commit(&bar_kfree[s]);
+                            if (i == n - 1) umma_commit(&bar_qfree);
                         }
                     }
-                    if (__any_sync(0xffffffffu, odd & 0x80008000u)) {
-                        odd_ring[seg % ODD_RING] = seg + 1;
-                        uint32_t *e = reinterpret_cast<uint32_t *>(v);
-                        for (int i = lane; i < TILE / 4; i += 32) e[i] &= ~((((e[i] & EXP) + ONE) >> 15 & 0x00010001u) * 0xffffu);
+                    __syncwarp();
+                };
+                auto issue_o = [&](int x, int i) {
+                    const int s = (tile + i) % NS;
+                    mbar_wait_nap(&bar_p[x][buffer(i)], (BUFS == 2 ? (uint32_t)(tile + i) >> 1 : n_p[x]) & 1u, fail, 0);
+                    if (i == 0 && x == 0 && seg > 0) mbar_wait_nap(&bar_od, (uint32_t)(seg - 1) & 1u, fail, 0);
+                    tc_fence_after();
+                    if (leader) {
+                        const uint64_t vd = desc_mn<KHALF>(su32(vs + s * TILE));
+    #pragma unroll
+                        for (int e = 0; e < KT / 16; e++)
+                            umma_f16_ta(tmem + O_COL + (uint32_t)(x * T), tmem + column(x, i) + (uint32_t)(e * 8), vd + (uint64_t)(e * 128), IDESC_PV, (i > (SHARE ? 0 : 1) || e) ? 1u : 0u);
+                        umma_commit(&bar_o[x][buffer(i)]);
+                        if (!SHARE || x == 1) umma_commit(&bar_vfree[s]);
+                    }
+                    __syncwarp();
+                    n_p[x]++;
+                };
+                auto wait_for = [&](uint64_t *bar, int i) { mbar_wait_nap(&bar[(tile + i) % NS], (uint32_t)((tile + i) / NS) & 1u, fail, 0); };
+                mbar_wait_nap(&bar_q, (uint32_t)seg & 1u, fail, 0);
+                // (taking a P that is ready before keys that are not, so that a tile of values is free sooner: 185 us against 177 at 48 x 4096)
+                constexpr int AHEAD = SHARE ? BUFS : 2;
+                for (int i = 0; i < min(AHEAD, n); i++) {
+                    wait_for(bar_k, i);
+                    issue_s(SHARE ? 0 : i, i);
+                    if (SHARE) issue_s(1, i);
+                }
+                for (int i = 0; i < n; i++) {
+                    const bool more = i + AHEAD < n;
+                    wait_for(bar_fix, i);
+                    issue_o(SHARE ? 0 : i & 1, i);
+                    if (more) {
+                        wait_for(bar_k, i + AHEAD);
+                        issue_s(SHARE ? 0 : i & 1, i + AHEAD);
+                    }
+                    if (SHARE) {
+                        issue_o(1, i);
+                        if (more) issue_s(1, i + AHEAD);
                     }
                 }
-                if (j >= g.special) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_fix[s]);
+                tile += n;
+                seg++;
             }
-            seg++;
+        } else if (warp == 2) {
+            // ---- every tile of values passes here, in order, on its way to the MMAs. Special ones: rows behind the end become zero, the others are
+            // looked through
+            int tile = 0, seg = 0;
+            while (next()) {
+                if (g.t1 == g.t0) continue;
+                for (int j = g.t0; j < g.t1; j++, tile++) {
+                    const int s = tile % NS;
+                    mbar_wait_nap(&bar_v[s], (uint32_t)(tile / NS) & 1u, fail, 0);
+                    if (j >= g.special) {
+                        const int live = min(KT, g.nk - j * KT);
+                        uint4 *v = reinterpret_cast<uint4 *>(vs + s * TILE);
+                        constexpr uint32_t EXP = BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = BF16 ? 0x00800080u : 0x04000400u;   // one more than all ones carries into the sign
+                        uint32_t odd = 0;
+    #pragma unroll 8
+                        for (int i = lane; i < TILE / 16; i += 32) {
+                            if (((i >> 3) & (KT - 1)) >= live) {
+                                v[i] = make_uint4(0, 0, 0, 0);
+                            } else {
+                                const uint4 w = v[i];
+                                odd |= ((w.x & EXP) + ONE) | ((w.y & EXP) + ONE) | ((w.z & EXP) + ONE) | ((w.w & EXP) + ONE);
+                            }
+                        }
+                        if (__any_sync(0xffffffffu, odd & 0x80008000u)) {
+                            odd_ring[seg % ODD_RING] = seg + 1;
+                            uint32_t *e = reinterpret_cast<uint32_t *>(v);
+                            for (int i = lane; i < TILE / 4; i += 32) e[i] &= ~((((e[i] & EXP) + ONE) >> 15 & 0x00010001u) * 0xffffu);
+                        }
+                    }
+                    if (j >= g.special) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar_fix[s]);
+                }
+                seg++;
+            }
+        } else if (warp == 3) {
+            int tile = 0;
+            while (next()) copy_tiles(vs, &p.v, bar_v, bar_vfree, tile, [](int) {}, [](int) {});
         }
-    } else if (warp == 3) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROLES));
-        int tile = 0;
-        while (next()) copy_tiles(vs, &p.v, bar_v, bar_vfree, tile, [](int) {}, [](int) {});
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_STREAMS));
         // ---- the streams

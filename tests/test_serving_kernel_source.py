@@ -1,0 +1,28 @@
+"""Rules that the attention kernel of k_serve_attn_tc.cu has to keep and that no run shows: read from its source."""
+import re
+from pathlib import Path
+
+CSRC = Path(__file__).resolve().parent.parent / "tensorlisp_b200" / "csrc"
+TEXT = (CSRC / "k_serve_attn_tc.cu").read_text()
+
+
+def conditions(text, at):
+    """The conditions of the blocks around a place of the source, from the outermost in ("else": of an if without another condition)."""
+    stack, begin = [], 0
+    for m in re.finditer(r"[{};]", text[:at]):
+        if m.group() == "{":
+            stack.append(re.sub(r"\s+", " ", re.sub(r"//[^\n]*", "", text[begin:m.start()])).strip())
+        elif m.group() == "}":
+            stack.pop()
+        begin = m.end()
+    return stack
+
+
+def test_register_shares_are_set_by_whole_warpgroups():
+    """All threads of a warpgroup have to execute the same setmaxnreg: it stands under conditions that are the same for four warps in a row."""
+    places = [m.start() for m in re.finditer(r'asm volatile\("setmaxnreg', TEXT)]
+    assert len(places) == 2
+    for at in places:
+        roles = [c for c in conditions(TEXT, at) if re.match(r"(if|else|for|while)\b", c)]
+        assert roles in (["if (warp < 4)"], ["else"]), roles
+    assert TEXT.index('"setmaxnreg.dec') < TEXT.index('"setmaxnreg.inc')
