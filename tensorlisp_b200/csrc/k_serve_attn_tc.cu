@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     constexpr uint32_t IDESC_QK = FMT | ((uint32_t)(KT >> 3) << 17), IDESC_PV = FMT | (1u << 16) | ((uint32_t)(HSP >> 3) << 17);
     extern __shared__ __align__(1024) uint8_t smem[];   // behind 3 KB of the arrays below, so that three stages fill the 227 KB to the byte
     uint8_t *qs = smem, *ks = qs + NQ * QTILE, *vs = ks + NS * TILE;
-    __shared__ uint64_t bar_q, bar_qfree, bar_k[NS], bar_kfree[NS], bar_v[NS], bar_vfree[NS], bar_fix[NS], bar_s[2][BUFS], bar_p[2][BUFS], bar_o[2][BUFS], bar_od;
+    __shared__ uint64_t bar_q, bar_qfree, bar_k[NS], bar_kfree[NS], bar_v[NS], bar_vfree[NS], bar_fix[NS], bar_s[2][BUFS], bar_p[2][BUFS], bar_o[2][BUFS], bar_od, bar_pair;
     __shared__ uint32_t tmem_base_s;
     __shared__ int s_fail;
     __shared__ volatile int odd_ring[ODD_RING];   // segment + 1 of those whose special tiles hold values that are not finite
@@ -485,6 +485,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             }
         }
         mbar_init(&bar_od, 8);
+        mbar_init(&bar_pair, 8);
         for (int i = 0; i < SEG_RING; i++) {
             mbar_init(&bar_seg[i], 1);
             mbar_init(&bar_segfree[i], 11);   // every warp but the one that writes
@@ -515,7 +516,8 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar_segfree[r]);
         g_at++;
-        return g.t0 >= 0 && !*fail;
+        g.t0 = __shfl_sync(0xffffffffu, g.t0, 0);   // a warp goes on or leaves as one, also where a wait gave up and what it read is half written
+        return g.t0 >= 0 && !__any_sync(0xffffffffu, *fail);
     };
 
     // The tiles of a segment on their way to a ring of stages (warp 0: keys, warp 3: values)
@@ -738,8 +740,14 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         const int x = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         const uint32_t s_at = lanes + (uint32_t)(x * T), o_at = lanes + O_COL + (uint32_t)(x * T);
-        int seg = 0;
+        int seg = 0, n_pair = 0;
         uint32_t done[2] = {0, 0};   // tiles of either stream so far
+        // The eight warps of both streams wait for one another, as bounded as every other wait: a warp that has left after a wait gave up arrives no more
+        auto pair_sync = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_pair);
+            mbar_wait_nap(&bar_pair, (uint32_t)n_pair++ & 1u, fail, 20);
+        };
         while (next()) {
             const int ctx = g.ctx();
             const int token = g.token0 + (SHARE ? x * p.tpt : 0) + row / p.group, head = g.kvh * p.group + row % p.group;
@@ -843,12 +851,12 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
             const int prow = (SHARE ? x * T : 0) + row;
             {
                 float f_mine = 1.f, f_other = 0.f;
-                if (!SHARE) {
+                if (!SHARE && n > 0) {
+                    // nobody is still reading what the segment in front left here: its O has come, and P V of a segment follows bar_od of the one in front
                     pair_ml[x][row][0] = have_ref ? m_ref : -CUDART_INF_F;
                     pair_ml[x][row][1] = l;
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    pair_sync();
                     const float m2 = pair_ml[x ^ 1][row][0], l2 = pair_ml[x ^ 1][row][1], m1 = have_ref ? m_ref : -CUDART_INF_F;
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
                     m_ref = fmaxf(m1, m2);
                     if (m_ref == -CUDART_INF_F) m_ref = 0.f;
                     f_mine = ex2(m1 - m_ref);
@@ -921,7 +929,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 if (odd) {
                     // the rows' results, some of them written by other lanes or (halves of the columns) the other stream's warps, are all there
                     if (SHARE) __syncwarp();
-                    else asm volatile("bar.sync 1, 256;" ::: "memory");
+                    else pair_sync();
                     if (PAGED && !have_bits) view.bits = ancestors_of(parents, token & 63, p.a.err);
                     if (view.lim >= 0 && (SHARE || x == 0)) add_odd_values<E, PAGED, KT>(p, g, view, token, head, m_ref, whole ? inv : 1.f, part, NQ * T, prow);
                     __syncwarp();

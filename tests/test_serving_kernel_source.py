@@ -26,3 +26,13 @@ def test_register_shares_are_set_by_whole_warpgroups():
         roles = [c for c in conditions(TEXT, at) if re.match(r"(if|else|for|while)\b", c)]
         assert roles in (["if (warp < 4)"], ["else"]), roles
     assert TEXT.index('"setmaxnreg.dec') < TEXT.index('"setmaxnreg.inc')
+
+
+def test_every_wait_inside_the_roles_is_bounded():
+    """Once a wait has given up, warps leave their roles at different places: between the first role and the barrier in front of the kernel's end nothing
+    may wait for a number of threads without a limit, and what is looked at of the others' failure has to be the same for a whole warp."""
+    a, b = TEXT.index('"setmaxnreg.dec'), TEXT.index("// only after a wait has given up")
+    roles = TEXT[TEXT.index("auto next = [&]"):b]
+    assert a < b and "bar.sync" not in roles and "barrier.sync" not in roles and "__syncthreads" not in roles
+    looks = re.findall(r"[^\n;{]*\*fail\b[^\n]*", roles)
+    assert looks and all("__any_sync(0xffffffffu, *fail" in x for x in looks), looks
