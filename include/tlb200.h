@@ -317,7 +317,7 @@ tlb_status tlb_cache_keep(tlb_device *dev, const tlb_cache_keep_args *args, void
 typedef struct tlb_token_logprobs_args {
     uint32_t type;                    /* TLB_TYPE_F32, TLB_TYPE_F16 or TLB_TYPE_BF16 */
     uint32_t top;
-    uint64_t rows, vocab;
+    uint64_t rows, vocab;             /* vocab: up to 2^31 - 2048 */
     const void *logits;               /* rows of vocab values */
     uint64_t stride;                  /* from row to row, a multiple of the value's size */
     const int32_t *tokens;            /* [rows]; NULL: none */

@@ -402,6 +402,7 @@ static lp::Scan lp_plan(const Logprobs &a, int sm_count, uint64_t *bytes) {
     lp::Scan p{};
     p.a = a;
     constexpr int64_t TURN = (int64_t)lp::Vec<T>::SEG * lp::UNROLL;
+    static_assert(LOGPROBS_MAX_VOCAB + TURN + lp::Vec<T>::N <= 0x7fffffff, "a turn that begins in front of the row's end ends below 2^31");
     p.turns = (int)((a.vocab + lp::Vec<T>::N - 1 + TURN - 1) / TURN);   // wherever in 16 bytes a row starts
     // Eight turns of every warp where there are rows enough for 24 CTAs per SM, down to one; with few rows, CTAs of fewer warps' turns
     int64_t per = 8 * lp::WARPS;

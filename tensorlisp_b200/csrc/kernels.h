@@ -357,6 +357,7 @@ cudaError_t launch_cache_keep(const CacheKeep &a, cudaStream_t st);
 // ---------------------------------------------------------------- k_logprobs.cu
 // Of each row of logits: log probability of a given token, entropy, the most likely tokens (ties: the lowest id) with theirs
 constexpr int LOGPROBS_MAX_TOP = 32;
+constexpr int64_t LOGPROBS_MAX_VOCAB = 0x7ffff800;   // places behind a row's end, up to what a warp loads at once (1024 values) and a piece, are 32-bit numbers too
 struct Logprobs {
     uint32_t type;                 // f32, f16 or bf16
     int64_t rows, vocab, stride;   // stride: bytes

@@ -134,7 +134,7 @@ Logprobs logprob_args(const tlb_token_logprobs_args &p) {
 const char *logprobs_refusal(const Logprobs &a) {
     if (a.type != TLB_TYPE_F32 && a.type != TLB_TYPE_F16 && a.type != TLB_TYPE_BF16) return "logits must be f32, f16 or bf16";
     if (a.top > LOGPROBS_MAX_TOP) return "at most 32 alternatives";
-    if (a.rows > 0x7fffffff || a.vocab < 1 || a.vocab > 0x7fffff00) return "1 to 2^31 - 257 tokens, up to 2^31 - 1 rows";
+    if (a.rows > 0x7fffffff || a.vocab < 1 || a.vocab > LOGPROBS_MAX_VOCAB) return "1 to 2^31 - 2048 tokens, up to 2^31 - 1 rows";
     return nullptr;
 }
 
