@@ -352,12 +352,11 @@ __device__ __forceinline__ uint32_t round2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-__device__ __forceinline__ void add2(uint64_t &s, float a, float b) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(pack2(a, b))); }
-__device__ __forceinline__ float total2(uint64_t s, uint64_t t) {
-    float a, b;
-    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(t));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(s));
-    return a + b;
+// a += low half of w, b += the high one
+template <bool BF16>
+__device__ __forceinline__ void add_halves(uint32_t w, float &a, float &b) {
+    if (BF16) asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.bf16 %0, l, %0;\n\tadd.rn.f32.bf16 %1, h, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(w));
+    else asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.f16 %0, l, %0;\n\tadd.rn.f32.f16 %1, h, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(w));
 }
 __device__ __forceinline__ void ld32(uint32_t taddr, float *x) {
     uint32_t *r = reinterpret_cast<uint32_t *>(x);
@@ -516,7 +515,13 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar_segfree[r]);
         g_at++;
-        g.t0 = __shfl_sync(0xffffffffu, g.t0, 0);   // a warp goes on or leaves as one, also where a wait gave up and what it read is half written
+        // A warp goes on or leaves as one, also where a wait gave up and what it read is half written. (Either form for both: trees 32 x 16 72 and 48 x 32 177 us
+        // against 66 and 160, 24 x 1000 68 and 1 x 8192 511 against 65 and 489)
+        if (PAGED) {
+            if (__any_sync(0xffffffffu, *fail)) g.t0 = -1;
+            return g.t0 >= 0;
+        }
+        g.t0 = __shfl_sync(0xffffffffu, g.t0, 0);
         return g.t0 >= 0 && !__any_sync(0xffffffffu, *fail);
     };
 
@@ -817,7 +822,6 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                     l *= alpha;
                 }
                 const uint64_t sc = pack2(p.scale_log2, p.scale_log2), ref = pack2(-m_ref, -m_ref);
-                uint64_t sums[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < KT / 64; c++) {
                     uint32_t w[32];
@@ -827,16 +831,23 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                         fma2(a, b, sc, ref);
                         a = ex2(a);
                         b = ex2(b);
-                        add2(sums[e & 1], a, b);
                         w[e] = round2<BF16>(a, b);
                     }
                     st32(s_at + b * KT + 32 * c, w);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) y[32 * c + e] = __uint_as_float(w[e]);
                 }
-                l += total2(sums[0], sums[1]);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_p[x][b]);
+                // The sums of P as it was rounded, while it is multiplied: O has the same roundings, so the weights add up to 1 however far the reference lags.
+                // Sums of the unrounded values: 24 x 1000 62 us against 65, chunks 72 against 74, 1 x 8192 472 against 488; with the reference lagging by up to 2^8 a dominant
+                // key's weight was off by up to 2^-8 in bf16. Within the loop of the exponentials: trees 74 and 185 us against 66 and 160
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < KT / 2; e++) add_halves<BF16>(__float_as_uint(y[e]), sum[2 * (e & 1)], sum[2 * (e & 1) + 1]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
             done[x] += mine;
             done[x ^ 1] += other;
