@@ -999,10 +999,14 @@ __global__ void __launch_bounds__(256) k_serve_join(const __grid_constant__ sat:
             for (int e = 0; e < W; e++) y[u][e] = s[(size_t)e * ROWS];
         }
         float top = m;
+        bool some = false;
 #pragma unroll
         for (int u = 0; u < 4; u++)
-            if (ml[u].y != 0.f) top = fmaxf(top, ml[u].x);   // l = 0: the row sees nothing in this part
-        if (top == -CUDART_INF_F) continue;
+            if (ml[u].y != 0.f) {   // l = 0: the row sees nothing in this part
+                top = fmaxf(top, ml[u].x);   // a NaN is passed over and comes in with the part's l
+                some = true;
+            }
+        if (!some) continue;
         const float keep = ex2(m - top);
         m = top;
         l *= keep;

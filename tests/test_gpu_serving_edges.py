@@ -36,3 +36,55 @@ def test_the_largest_vocabulary(native, dtype, first):
     assert ids.tolist() == [[i for _, i in want]]
     assert abs(lp.item() - (3.0 - lse)) < 2.0 ** -20 and abs(ent.item() - sum(math.exp(-d) * d for d, _ in want)) < 2.0 ** -19
     assert np.abs(top.cpu().numpy()[0] + [d for d, _ in want]).max() < 2.0 ** -20
+
+
+def randn(shape, seed, dtype=torch.float16):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+def packed(native, q, k, v, q_at, kv_at=None):
+    out = torch.full_like(q, 77.0)
+    ws = room(ops.packed_attention_workspace(native, q, k, len(q_at) - 1))
+    ops.packed_attention(native, q, k, v, i32(q_at), out, kv_offsets=None if kv_at is None else i32(kv_at), workspace=ws, stream=torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    return out
+
+
+def tree(native, q, k_pool, v_pool, tables, context, counts, parents):
+    out = torch.full_like(q, 77.0)
+    ws = room(ops.tree_attention_workspace(native, q, k_pool, tables))
+    ops.tree_attention(native, q, k_pool, v_pool, tables, context, counts, parents, out, workspace=ws, stream=torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    return out
+
+
+# Row tiles over many keys are cut between CTAs, so parts of the rows are joined by a launch behind: in the first, third and last of these
+SHAPES = [([3000], None), ([40], None), ([300, 1, 200], [4000, 1, 1000]), ([2, 5], [3, 600]), ([1], [20000])]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens,keys", SHAPES)
+def test_a_query_that_is_no_number(native, lens, keys, D):
+    """Every weight of its row is NaN and so is its result; the other rows and heads have theirs, to the last bit."""
+    q_at, kv_at = [0] + list(np.cumsum(lens)), [0] + list(np.cumsum(keys or lens))
+    q, k, v = randn((q_at[-1], 4, D), 1), randn((kv_at[-1], 1, D), 2), randn((kv_at[-1], 1, D), 3)
+    want = packed(native, q, k, v, q_at, kv_at)
+    rows = sorted({0, q_at[-1] // 2, q_at[-1] - 1})
+    for i in rows:
+        q[i, i % 4, D // 3] = float("nan")
+        want[i, i % 4] = float("nan")
+    out = packed(native, q, k, v, q_at, kv_at)
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[~torch.isnan(want)], want[~torch.isnan(want)])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("ctx", [10, 3000])
+def test_a_draft_that_is_no_number(native, ctx, D):
+    pages = -(-(ctx + 8) // 16)
+    q, kp, vp = randn((1, 8, 4, D), 4), randn((pages, 2, 16, D), 5), randn((pages, 2, 16, D), 6)
+    numbers = i32(np.random.default_rng(7).permutation(pages)[None]), i32([ctx]), i32([8]), i32([[-1, 0, 0, 1, 3, -1, 5, 2]])
+    want = tree(native, q, kp, vp, *numbers)
+    q[0, 5, 2, 7] = float("nan")
+    want[0, 5, 2] = float("nan")
+    out = tree(native, q, kp, vp, *numbers)
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[~torch.isnan(want)], want[~torch.isnan(want)])
