@@ -257,6 +257,7 @@ tlb_status tlb_paged_attention_static(tlb_device *dev, const void *q, const void
 /* Causal attention over packed sequences: sequence s has the query rows q_offsets[s] .. q_offsets[s + 1] and the key rows kv_offsets[s] ..
  * kv_offsets[s + 1]; its last query sees all of its keys, the one before it one less, ... (as many keys as queries: a prompt; more: a chunk
  * behind keys of earlier tokens; fewer: the first queries see nothing and give zeros). Query head h reads KV head h / (heads / kv_heads).
+ * What is not finite follows the formula: scores of -inf have no weight beside others, a row of nothing else and one with a score of NaN or +inf are NaN.
  * Head sizes: multiples of 8 up to 512 (tuned up to 128). Rows outside every sequence stay as they were, and so do those of a sequence whose
  * offsets fall or reach outside the rows (reported). */
 typedef struct tlb_packed_attention_args {

@@ -27,6 +27,7 @@ __global__ void __launch_bounds__(128) k_serve_attn_any(const ServeAttn a) {
     griddep_wait();
     constexpr int WARPS = 4;
     __shared__ float ml[WARPS][2];
+    __shared__ bool sees[WARPS];
     __shared__ float accs[WARPS][C * 256];
     __shared__ int seq_s;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -67,11 +68,13 @@ __global__ void __launch_bounds__(128) k_serve_attn_any(const ServeAttn a) {
         for (int e = 0; e < 8; e++) acc[c][e] = 0.f;
     }
     float m_run = -CUDART_INF_F, l_run = 0.f;
+    bool some = false;
     const float scale_log2 = a.scale * 1.4426950408889634f;
     for (int64_t key = warp; key < keys; key += WARPS) {
         if (PAGED && key >= ctx && !((bits >> (key - ctx)) & 1)) continue;
         const ServeRow at = serve_kv_row<PAGED>(a, seq, sq, kvh, key);
         if (!at.k) continue;
+        some = true;
         uint4 vraw[C];
         float dot = 0.f;
 #pragma unroll
@@ -106,6 +109,7 @@ __global__ void __launch_bounds__(128) k_serve_attn_any(const ServeAttn a) {
     if (lane == 0) {
         ml[warp][0] = m_run;
         ml[warp][1] = l_run;
+        sees[warp] = some;
     }
 #pragma unroll
     for (int c = 0; c < C; c++)
@@ -119,13 +123,15 @@ __global__ void __launch_bounds__(128) k_serve_attn_any(const ServeAttn a) {
     T *dst = reinterpret_cast<T *>((char *)a.out + (int64_t)row * a.out_stride) + (int64_t)head * a.hs;
     for (int d = threadIdx.x; d < a.hs; d += 128) {
         float l = 0.f, o = 0.f;
+        bool any = false;
 #pragma unroll
         for (int w = 0; w < WARPS; w++) {
+            any |= sees[w];
             const float f = exp2f(ml[w][0] - mu);   // 0 for a warp without a key
             l += ml[w][1] * f;
             o += accs[w][d] * f;
         }
-        dst[d] = serve_round<T>(l == 0.f ? 0.f : o / l);
+        dst[d] = serve_round<T>(any ? o / l : 0.f);   // l = 0 of a row that sees keys: nothing but scores of -inf, 0 / 0
     }
 }
 

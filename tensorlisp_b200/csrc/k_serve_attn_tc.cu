@@ -77,8 +77,8 @@ struct Place {
 struct Cut {
     int parts;      // 0: none
     int kvh, token0;
-    int q0, nq;     // the sequence's queries
-    int pad[3];
+    int q0, nq, ctx;   // the sequence's queries, keys in front of the first one's own
+    int pad[2];
 };
 struct Params {
     CUtensorMap q, k, v;
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                 const int64_t off = walk.at.off;
                 if (walk.left == 0 && off > 0 && off <= stretch) {   // further than the stretch is long: it begins in one in front
                     const int n = key_tiles<PAGED, KT>(p, walk.sq, walk.at.r);
-                    if (off < n) cut = {1 + (int)divide(n - off + share - 1, share), walk.at.kvh, walk.at.r * p.tt, (int)walk.sq.q0, walk.sq.nq, {}};
+                    if (off < n) cut = {1 + (int)divide(n - off + share - 1, share), walk.at.kvh, walk.at.r * p.tt, (int)walk.sq.q0, walk.sq.nq, (int)(walk.sq.nk - walk.sq.nq), {}};
                 }
                 p.cuts[blockIdx.x] = cut;
             }
@@ -875,7 +875,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
                     l = l * f_mine + l2 * f_other;
                 }
                 if (view.lim < 0) l = 0.f;   // a row that sees nothing, or no token's
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const float inv = view.lim < 0 ? 0.f : 1.f / l;   // l = 0 of one that does: nothing but scores of -inf, 0 / 0
                 if (whole) {
                     f_mine *= inv;
                     f_other *= inv;
@@ -1021,7 +1021,7 @@ __global__ void __launch_bounds__(256) k_serve_join(const __grid_constant__ sat:
             for (int e = 0; e < W; e++) o[e] = make_float4(fmaf(y[u][e].x, f, o[e].x), fmaf(y[u][e].y, f, o[e].y), fmaf(y[u][e].z, f, o[e].z), fmaf(y[u][e].w, f, o[e].w));
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = (PAGED ? token >= cut.nq : cut.ctx + token < 0) ? 0.f : 1.f / l;   // a row that sees nothing; l = 0 of one that does: 0 / 0
     char *dst = (char *)p.a.out + (int64_t)(cut.q0 + token) * p.a.out_stride + (int64_t)head * p.a.hs * 2;
 #pragma unroll
     for (int e = 0; e < W; e += 2) {

@@ -88,3 +88,51 @@ def test_a_draft_that_is_no_number(native, ctx, D):
     want[0, 5, 2] = float("nan")
     out = tree(native, q, kp, vp, *numbers)
     assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[~torch.isnan(want)], want[~torch.isnan(want)])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf")])
+@pytest.mark.parametrize("lens,keys", SHAPES + [([5], [3])])
+def test_a_query_with_an_infinite_value(native, lens, keys, bad, D):
+    """Its scores are infinite, of either sign: the weights are exp(inf - inf), or 0 / 0 where all are -inf. A row that sees nothing is zero all the same."""
+    q_at, kv_at = [0] + list(np.cumsum(lens)), [0] + list(np.cumsum(keys or lens))
+    q, k, v = randn((q_at[-1], 4, D), 1), randn((kv_at[-1], 1, D), 2), randn((kv_at[-1], 1, D), 3)
+    assert (k != 0).all()
+    want = packed(native, q, k, v, q_at, kv_at)
+    sees = torch.cat([torch.arange(n) + (m - n) >= 0 for n, m in zip(lens, keys or lens)]).cuda()
+    for i in sorted({0, q_at[-1] // 2, q_at[-1] - 1}):
+        q[i, i % 4, D // 3] = bad
+        want[i, i % 4] = float("nan") if sees[i] else 0.0
+    out = packed(native, q, k, v, q_at, kv_at)
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[~torch.isnan(want)], want[~torch.isnan(want)])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("behind", [0, 1000])
+def test_keys_of_infinite_distance(native, behind, D):
+    """Scores of -inf beside others have no weight; where a row has no other, its result is 0 / 0."""
+    n = 200
+    q, k, v = randn((n, 4, D), 1).abs(), randn((behind + n, 1, D), 2), randn((behind + n, 1, D), 3)
+    q[:, :, 5] = 1.0
+    k[:behind + 90, 0, 5] = -float("inf")
+    want = packed(native, q, k.clamp(min=-65504), v, [0, n], [0, behind + n])
+    out = packed(native, q, k, v, [0, n], [0, behind + n])
+    assert torch.isnan(out[:90]).all() and torch.equal(out[90:], want[90:])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("ctx", [10, 3000])
+def test_a_draft_whose_scores_are_infinite(native, ctx, D):
+    pages = -(-(ctx + 8) // 16)
+    q, kp, vp = randn((1, 8, 4, D), 4), randn((pages, 2, 16, D), 5), randn((pages, 2, 16, D), 6)
+    numbers = i32(np.random.default_rng(7).permutation(pages)[None]), i32([ctx]), i32([7]), i32([[-1, 0, 0, 1, 3, -1, 5, 2]])
+    want = tree(native, q, kp, vp, *numbers)
+    assert (want[0, 7] == 0).all()
+    q[0, 5, 2, 7], q[0, 7, 1, 7] = float("inf"), float("inf")      # the last one is padding
+    want[0, 5, 2] = float("nan")
+    out = tree(native, q, kp, vp, *numbers)
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[~torch.isnan(want)], want[~torch.isnan(want)])
+    kp[:, :, :, 3] = -float("inf")
+    q = q.abs().clamp(min=0.5)
+    out = tree(native, q, kp, vp, *numbers)
+    assert torch.isnan(out[0, :7]).all() and (out[0, 7] == 0).all()
