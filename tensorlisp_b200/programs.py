@@ -443,12 +443,16 @@ class TreeDecodeLoop:
         path, gained = np.zeros((B, D), np.int32), []
         kept = np.ones(B, np.int32)
         for b in range(B):
-            at, new = 0, [int(follows[b, 0])]
-            for i in range(1, int(counts[b])):      # drafts come behind their parents
-                if parents[b, i] == at and ids[b, i] == new[-1]:
-                    at = path[b, kept[b]] = i
-                    kept[b] += 1
-                    new.append(int(follows[b, i]))
+            best, agrees = 0, [True] * int(counts[b])
+            for i in range(1, int(counts[b])):      # drafts come behind their parents; the same token may follow one twice
+                agrees[i] = agrees[parents[b, i]] and ids[b, i] == follows[b, parents[b, i]]
+                if agrees[i] and depth[b, i] > depth[b, best]:
+                    best = i
+            kept[b] = depth[b, best] + 1
+            at = best
+            for j in range(int(depth[b, best]), 0, -1):
+                path[b, j], at = at, parents[b, at]
+            new = [int(t) for t in ids[b, path[b, 1:kept[b]]]] + [int(follows[b, best])]
             gained.append(new)
         self._keep(path, kept)
         self.context = self.context + kept
