@@ -252,7 +252,8 @@ tlb_status tlb_paged_attention_static(tlb_device *dev, const void *q, const void
  * that the _workspace function gives for the same shapes) needs no initial content; calls that may overlap in time need one each.
  * Shapes and alignments are checked (TLB_INVALID, TLB_UNSUPPORTED); numbers in device memory are checked where they are read: one that
  * points outside is not followed, and *status (device or pinned memory, may be NULL, never reset) becomes 4; it becomes 2 if a kernel gave up
- * waiting for its own copies. What a call writes, workspace and status among it, may not overlap anything else that it is given. */
+ * waiting for its own copies. What a call writes, workspace and status among it, may not overlap anything else that it is given
+ * (column blocks of one wide buffer do not; strided arrays of different steps count from their first byte to their last). */
 
 /* Causal attention over packed sequences: sequence s has the query rows q_offsets[s] .. q_offsets[s + 1] and the key rows kv_offsets[s] ..
  * kv_offsets[s + 1]; its last query sees all of its keys, the one before it one less, ... (as many keys as queries: a prompt; more: a chunk

@@ -28,17 +28,30 @@ bool overlap(const void *p, uint64_t n, const void *q, uint64_t m) {
     const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
     return p && q && n && m && a < b + m && b < a + n;
 }
+// rows of `n` bytes, `stride` bytes apart; a dense array is one row
 struct Range {
     const void *p;
     uint64_t n;
+    uint64_t rows = 1, stride = 0;
+    uint64_t span() const { return rows ? (rows - 1) * stride + n : 0; }
 };
+// Rows with one step, and a row beside others, share a byte unless each lies in the other's gaps: columns of one wide buffer do not. Different steps:
+// judged by where the arrays begin and end.
+bool share(const Range &a, const Range &b) {
+    if (!overlap(a.p, a.span(), b.p, b.span())) return false;
+    if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) return true;
+    const uint64_t step = a.rows > 1 ? a.stride : b.stride;
+    if ((a.rows == 1 && b.rows == 1) || step == 0 || a.n > step || b.n > step) return true;
+    const uint64_t x = (uintptr_t)a.p % step, y = (uintptr_t)b.p % step, d = y >= x ? y - x : y + step - x;   // from a row of a to the next of b
+    return d < a.n || step - d < b.n;
+}
 // what a call writes shares no byte with anything else of it
 bool clash(std::initializer_list<Range> writes, std::initializer_list<Range> reads) {
     for (const Range *w = writes.begin(); w != writes.end(); w++) {
         for (const Range *x = w + 1; x != writes.end(); x++)
-            if (overlap(w->p, w->n, x->p, x->n)) return true;
+            if (share(*w, *x)) return true;
         for (const Range &r : reads)
-            if (overlap(w->p, w->n, r.p, r.n)) return true;
+            if (share(*w, r)) return true;
     }
     return false;
 }
@@ -48,7 +61,6 @@ bool numbers(std::initializer_list<const void *> arrays) {
     return true;
 }
 const char *const NUMBERS = "numbers must lie on 4-byte boundaries", *const CLASH = "a result or the workspace overlaps another array";
-uint64_t span(uint64_t rows, uint64_t stride, uint64_t row) { return rows ? (rows - 1) * stride + row : 0; }
 bool product_fits(std::initializer_list<uint64_t> f) {
     unsigned __int128 n = 1;
     for (uint64_t x : f) {
@@ -165,9 +177,9 @@ tlb_status tlb_packed_attention(tlb_device *dev, const tlb_packed_attention_args
     for (uint64_t rows : {(uint64_t)a.q_rows, (uint64_t)a.kv_rows})
         if (!product_fits({rows, std::max({args->q_stride, args->k_stride, args->v_stride, args->out_stride})})) return fail(TLB_INVALID, me + "sizes overflow");
     const uint64_t need = serve_attn_scratch_bytes(a, dev->prop.multiProcessorCount), off = ((uint64_t)a.seqs + 1) * 4;
-    if (clash({{a.out, span(a.q_rows, args->out_stride, q_row)}, {args->workspace, need}, {a.err, 4}},
-              {{a.q, span(a.q_rows, args->q_stride, q_row)}, {a.k, span(a.kv_rows, args->k_stride, kv_row)}, {a.v, span(a.kv_rows, args->v_stride, kv_row)},
-               {a.q_off, off}, {a.kv_off, off}}))
+    const uint64_t q_rows = (uint64_t)a.q_rows, kv_rows = (uint64_t)a.kv_rows;
+    if (clash({{a.out, q_row, q_rows, args->out_stride}, {args->workspace, need}, {a.err, 4}},
+              {{a.q, q_row, q_rows, args->q_stride}, {a.k, kv_row, kv_rows, args->k_stride}, {a.v, kv_row, kv_rows, args->v_stride}, {a.q_off, off}, {a.kv_off, off}}))
         return fail(TLB_INVALID, me + CLASH);
     if (need && (!args->workspace || args->workspace_bytes < need || !aligned(args->workspace, 16)))
         return fail(TLB_INVALID, me + "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed, got " + std::to_string(args->workspace ? args->workspace_bytes : 0));
@@ -219,16 +231,8 @@ tlb_status tlb_cache_keep(tlb_device *dev, const tlb_cache_keep_args *args, void
     const uint64_t pool = p.pool_blocks * page;
     if (!aligned(p.k_pools, 16) || !aligned(p.v_pools, 16) || p.k_layer_stride % 16 || p.v_layer_stride % 16 || p.k_layer_stride >> 46 || p.v_layer_stride >> 46)
         return fail(TLB_INVALID, me + "pools must start on 16-byte boundaries");
-    bool both = p.layers > 1 && (p.k_layer_stride < pool || p.v_layer_stride < pool);
-    if (!both && overlap(p.k_pools, span(p.layers, p.k_layer_stride, pool), p.v_pools, span(p.layers, p.v_layer_stride, pool))) {
-        // keys and values of the layers in turn: the same step, and room for one beside the other
-        const uint64_t step = p.k_layer_stride;
-        both = p.layers == 1 || step != p.v_layer_stride;
-        if (!both) {
-            const uint64_t k = (uintptr_t)p.k_pools % step, v = (uintptr_t)p.v_pools % step, d = v >= k ? v - k : v + step - k;
-            both = d < pool || step - d < pool;
-        }
-    }
+    const Range keys{p.k_pools, pool, p.layers, p.k_layer_stride}, values{p.v_pools, pool, p.layers, p.v_layer_stride};
+    const bool both = (p.layers > 1 && (p.k_layer_stride < pool || p.v_layer_stride < pool)) || share(keys, values);
     if (both) return fail(TLB_INVALID, me + "two pools overlap");
     if (!numbers({p.tables, p.context, p.counts, p.path, p.status})) return fail(TLB_INVALID, me + NUMBERS);
     CacheKeep a{};
@@ -271,7 +275,7 @@ tlb_status tlb_token_logprobs(tlb_device *dev, const tlb_token_logprobs_args *ar
     if (!numbers({a.tokens, a.logprob, a.entropy, a.top_ids, a.top_logprobs, a.err})) return fail(TLB_INVALID, me + NUMBERS);
     if (!product_fits({(uint64_t)a.rows, args->stride})) return fail(TLB_INVALID, me + "sizes overflow");
     const uint64_t need = logprobs_scratch_bytes(a, dev->prop.multiProcessorCount), n = (uint64_t)a.rows * 4, nk = n * a.top;
-    if (clash({{a.logprob, n}, {a.entropy, n}, {a.top_ids, nk}, {a.top_logprobs, nk}, {args->workspace, need}, {a.err, 4}}, {{a.logits, span(a.rows, args->stride, row)}, {a.tokens, n}}))
+    if (clash({{a.logprob, n}, {a.entropy, n}, {a.top_ids, nk}, {a.top_logprobs, nk}, {args->workspace, need}, {a.err, 4}}, {{a.logits, row, (uint64_t)a.rows, args->stride}, {a.tokens, n}}))
         return fail(TLB_INVALID, me + CLASH);
     if (!args->workspace || args->workspace_bytes < need || !aligned(args->workspace, 16))
         return fail(TLB_INVALID, me + "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed, got " + std::to_string(args->workspace ? args->workspace_bytes : 0));

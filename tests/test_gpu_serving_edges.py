@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from tensorlisp_b200 import device_ops as ops
+from tensorlisp_b200._lib import TlbError
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +137,20 @@ def test_a_draft_whose_scores_are_infinite(native, ctx, D):
     q = q.abs().clamp(min=0.5)
     out = tree(native, q, kp, vp, *numbers)
     assert torch.isnan(out[0, :7]).all() and (out[0, 7] == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_result_beside_its_operands(native, D):
+    """Queries, keys, values and the result are column blocks of one buffer: no byte of the result is one of theirs."""
+    H, Gr, rows = 4, 2, 300
+    wide = randn((rows, 2 * H + 2 * Gr, D), 8)
+    q, k, v, out = wide[:, :H], wide[:, H:H + Gr], wide[:, H + Gr:H + 2 * Gr], wide[:, H + 2 * Gr:]
+    want, before = packed(native, q.contiguous(), k.contiguous(), v.contiguous(), [0, 40, 300]), wide.clone()
+    ws = room(ops.packed_attention_workspace(native, q, k, 2))
+    go = lambda o: ops.packed_attention(native, q, k, v, i32([0, 40, 300]), o, workspace=ws, stream=torch.cuda.current_stream())  # noqa: E731
+    go(out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(wide[:, :H + 2 * Gr], before[:, :H + 2 * Gr])
+    for o in (q, wide[:, H - 1:2 * H - 1], wide[:, 1:H + 1], wide[:, H + 2 * Gr - 1:-1]):
+        with pytest.raises(TlbError):
+            go(o)
