@@ -1020,6 +1020,8 @@ static const char *serve_attn_args(const Graph &g, const Tensor &t, ServeAttn &a
     a.paged = paged;
     a.bf16 = q.ty == TLB_TYPE_BF16;
     a.scale = t.param_f32(0);
+    for (int i = 0; i < 4; i++)   // what is held in 32 bits below
+        if (q.ne[i] > 0x7fffffff || (!paged && (k.ne[i] > 0x7fffffff || v.ne[i] > 0x7fffffff))) return "more than 2^31 - 256 rows";
     a.hs = (int)q.ne[0];
     a.heads = (int)q.ne[1];
     if (t.ty != q.ty || k.ty != q.ty || v.ty != q.ty || (q.ty != TLB_TYPE_F16 && q.ty != TLB_TYPE_BF16)) return "queries, keys, values and result must all be f16 or all bf16";
@@ -1037,7 +1039,8 @@ static const char *serve_attn_args(const Graph &g, const Tensor &t, ServeAttn &a
         if (!numbers(3, (int64_t)a.max_blocks * a.seqs) || !numbers(4, a.seqs) || !numbers(5, a.seqs) || !numbers(6, (int64_t)a.drafts * a.seqs))
             return "block tables, context lengths, counts and parents must be contiguous i32, one row or number per sequence";
         if (a.kv_heads < 1 || a.block_size < 1 || a.hs < 1) return "the query heads must be a multiple of the kv heads";
-        a.pool_blocks = std::min(k.nelements(), v.nelements()) / ((int64_t)a.kv_heads * a.block_size * a.hs);
+        const unsigned __int128 page = (unsigned __int128)a.kv_heads * a.block_size * a.hs, pool = std::min(k.nelements(), v.nelements());
+        a.pool_blocks = (int64_t)(pool / page);
         a.q_rows = (int64_t)a.drafts * a.seqs;
         a.q_stride = a.out_stride = (int64_t)a.heads * a.hs * 2;
     } else {

@@ -6,7 +6,9 @@ import pytest
 import torch
 
 from tensorlisp_b200 import device_ops as ops
+from tensorlisp_b200 import graph as G
 from tensorlisp_b200._lib import TlbError
+from tensorlisp_b200.native import Native, NativeProgram
 
 pytestmark = pytest.mark.gpu
 
@@ -154,3 +156,31 @@ def test_a_result_beside_its_operands(native, D):
     for o in (q, wide[:, H - 1:2 * H - 1], wide[:, 1:H + 1], wide[:, H + 2 * Gr - 1:-1]):
         with pytest.raises(TlbError):
             go(o)
+
+
+def test_nodes_of_impossible_sizes_are_refused():
+    """KV heads x tokens of a page x head size that pass 64 bits, sizes that pass 32: refusals of the compiler."""
+    n = Native.load([])
+    n.alloc_states([1 << 17, 1 << 17])
+
+    def refused(change, word, block_size=16):
+        g = G.Graph()
+        q, kc, vc = g.input(G.F16, [16, 4, 8, 2], "q"), g.state(G.F16, [1 << 16], "k"), g.state(G.F16, [1 << 16], "v")
+        ins = [g.input(G.I32, x, "x") for x in ([4, 2], [2], [2], [8, 2])]
+        y = g.output(g.paged_tree_attention(q, kc, vc, *ins, block_size, 0.25, 4))
+        change(g.tensors[y])
+        with pytest.raises(TlbError) as e:
+            NativeProgram.compile(n, g)
+        assert e.value.kind == "Unsupported" and word in str(e.value), str(e.value)
+
+    def kv_heads(x):
+        def change(t):
+            t.op_params[1] = x
+        return change
+
+    refused(kv_heads(1 << 30), "kv heads", 1 << 30)     # 2^64 values a page
+    refused(kv_heads(1 << 30), "kv heads", 3)
+    refused(kv_heads(0), "kv heads")
+    refused(kv_heads(4), "2^31", 1 << 30)
+    refused(kv_heads(4), "power of two", 24)
+    n.close()
