@@ -235,6 +235,8 @@ tlb_status tlb_cache_keep(tlb_device *dev, const tlb_cache_keep_args *args, void
     const bool both = (p.layers > 1 && (p.k_layer_stride < pool || p.v_layer_stride < pool)) || share(keys, values);
     if (both) return fail(TLB_INVALID, me + "two pools overlap");
     if (!numbers({p.tables, p.context, p.counts, p.path, p.status})) return fail(TLB_INVALID, me + NUMBERS);
+    const uint64_t n = (uint64_t)p.seqs * 4;
+    if (clash({keys, values, {p.status, 4}}, {{p.tables, n * p.max_blocks}, {p.context, n}, {p.counts, n}, {p.path, n * p.drafts}})) return fail(TLB_INVALID, me + CLASH);
     CacheKeep a{};
     a.kpool = p.k_pools;
     a.vpool = p.v_pools;

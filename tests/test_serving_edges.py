@@ -36,3 +36,14 @@ def test_pools_of_layers_in_turn():
         call("tlb_cache_keep", keep(tables=A[4] + 2, **fine), "4-byte", "Invalid")
     for bad in (dict(v_pools=A[0] + pool - 16), dict(v_pools=A[0] + 2 * pool + 16), dict(v_pools=A[0] + pool, v_layer_stride=3 * pool), dict(v_pools=A[0] + 2 * pool, k_layer_stride=pool, v_layer_stride=pool)):
         call("tlb_cache_keep", keep(**bad), "overlap", "Invalid")
+
+
+def test_numbers_inside_the_pools_are_refused():
+    """What cache_keep moves could overwrite the tables and paths that say where to."""
+    pool = 20 * 2 * 16 * 64 * 2
+    for name in ("tables", "context", "counts", "path", "status"):
+        for at in (A[0] + 64, A[0] + pool + 4096, A[0] + 6 * pool - 4):
+            call("tlb_cache_keep", keep(**{name: at}), "overlap", "Invalid")
+    call("tlb_cache_keep", keep(status=A[4] + 8), "overlap", "Invalid")
+    # between the layers there is room
+    call("tlb_cache_keep", keep(k_layer_stride=4 * pool, v_layer_stride=4 * pool, context=A[0] + 2 * pool, counts=A[0] + 4 * pool - 8, tables=A[4] + 2), "4-byte", "Invalid")
