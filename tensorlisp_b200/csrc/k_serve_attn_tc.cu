@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(sat::THREADS, 1) k_serve_attn_tc(const __grid_
     constexpr int QTILE = T * HSP * 2, QHALF = T * 128, TILE = KT * HSP * 2, KHALF = KT * 128;   // bytes; halves: 64 columns
     constexpr uint32_t FMT = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(T >> 4) << 24);
     constexpr uint32_t IDESC_QK = FMT | ((uint32_t)(KT >> 3) << 17), IDESC_PV = FMT | (1u << 16) | ((uint32_t)(HSP >> 3) << 17);
-    extern __shared__ __align__(1024) uint8_t smem[];   // behind 3 KB of the arrays below, so that three stages fill the 227 KB to the byte
+    extern __shared__ __align__(1024) uint8_t smem[];   // behind up to 3 KB of the arrays below: with six stages of 64 keys of 128 values the 227 KB are full
     uint8_t *qs = smem, *ks = qs + NQ * QTILE, *vs = ks + NS * TILE;
     __shared__ uint64_t bar_q, bar_qfree, bar_k[NS], bar_kfree[NS], bar_v[NS], bar_vfree[NS], bar_fix[NS], bar_s[2][BUFS], bar_p[2][BUFS], bar_o[2][BUFS], bar_od, bar_pair;
     __shared__ uint32_t tmem_base_s;
@@ -1033,10 +1033,11 @@ __global__ void __launch_bounds__(256) k_serve_join(const __grid_constant__ sat:
 }
 
 // ---------------------------------------------------------------- host side
-// The register shares must not exceed what a CTA is launched with, or the streams would wait for theirs for good (serve_attn_tc_configure).
-static bool g_sat_registers = true;
+// The register shares must not exceed what a CTA is launched with, or the streams would wait for theirs for good, and shared memory of both kinds has to fit
+// (serve_attn_tc_configure).
+static bool g_sat_fits = true;
 bool serve_attn_tc_supported(const ServeAttn &a) {
-    if (!g_sat_registers || !tc_available() || a.hs > 128 || a.heads / a.kv_heads > sat::T) return false;
+    if (!g_sat_fits || !tc_available() || a.hs > 128 || a.heads / a.kv_heads > sat::T) return false;
     if (a.paged) return a.block_size >= 8 && a.pool_blocks > 0 && a.pool_blocks * a.kv_heads * a.block_size < 0x7fffffff;
     return a.kv_rows > 0;
 }
@@ -1072,9 +1073,15 @@ static cudaError_t sat_launch(const sat::Params &p, int ctas, cudaStream_t st) {
 template <int HSP, bool BF16, bool PAGED, bool SHARE>
 static void sat_configure() {
     cudaFuncAttributes at;
-    if (cudaFuncGetAttributes(&at, k_serve_attn_tc<HSP, BF16, PAGED, SHARE>) != cudaSuccess || at.numRegs * sat::THREADS < 128 * sat::REGS_ROLES + 256 * sat::REGS_STREAMS)
-        g_sat_registers = false;
-    cudaFuncSetAttribute(k_serve_attn_tc<HSP, BF16, PAGED, SHARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, sat::smem_bytes(HSP, SHARE));
+    int device, room;
+    const int tiles = sat::smem_bytes(HSP, SHARE);
+    if (cudaFuncGetAttributes(&at, k_serve_attn_tc<HSP, BF16, PAGED, SHARE>) != cudaSuccess || cudaGetDevice(&device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&room, cudaDevAttrMaxSharedMemoryPerBlockOptin, device) != cudaSuccess || at.numRegs * sat::THREADS < 128 * sat::REGS_ROLES + 256 * sat::REGS_STREAMS ||
+        ((int)at.sharedSizeBytes + 1023) / 1024 * 1024 + tiles > room ||
+        cudaFuncSetAttribute(k_serve_attn_tc<HSP, BF16, PAGED, SHARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, tiles) != cudaSuccess) {
+        cudaGetLastError();
+        g_sat_fits = false;
+    }
 }
 void serve_attn_tc_configure() {
     sat_configure<64, false, false, false>();

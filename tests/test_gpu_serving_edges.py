@@ -184,3 +184,14 @@ def test_nodes_of_impossible_sizes_are_refused():
     refused(kv_heads(4), "2^31", 1 << 30)
     refused(kv_heads(4), "power of two", 24)
     n.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("D", [8, 64, 72, 128])
+def test_head_sizes_up_to_128_are_on_the_tensor_cores(native, D, dtype):
+    """The kernel that is not turned off where it does not fit: it alone asks for scratch memory."""
+    for rows in (3, 900):
+        q, k = torch.empty((rows, 4, D), dtype=dtype, device="cuda"), torch.empty((rows, 2, D), dtype=dtype, device="cuda")
+        assert ops.packed_attention_workspace(native, q, k, 1) > 0
+    q, kp = torch.empty((2, 4, 4, D), dtype=torch.float16, device="cuda"), torch.empty((9, 2, 16, D), dtype=torch.float16, device="cuda")
+    assert ops.tree_attention_workspace(native, q, kp, torch.empty((2, 4), dtype=torch.int32, device="cuda")) > 0

@@ -36,3 +36,12 @@ def test_every_wait_inside_the_roles_is_bounded():
     assert a < b and "bar.sync" not in roles and "barrier.sync" not in roles and "__syncthreads" not in roles
     looks = re.findall(r"[^\n;{]*\*fail\b[^\n]*", roles)
     assert looks and all("__any_sync(0xffffffffu, *fail" in x for x in looks), looks
+
+
+def test_a_launch_that_does_not_fit_turns_the_kernel_off():
+    """Registers and shared memory (static and dynamic, each instance's own) are looked at where the kernel is set up, and so is whether that worked:
+    calls then go to the plain kernel instead of failing at the launch."""
+    body = TEXT[TEXT.index("static void sat_configure()"):TEXT.index("void serve_attn_tc_configure()")]
+    assert "numRegs" in body and "sharedSizeBytes" in body and "cudaDevAttrMaxSharedMemoryPerBlockOptin" in body
+    assert not re.search(r"^\s*cuda\w+\(.*\);$", body.replace("cudaGetLastError();", ""), re.M), "a result that nobody looks at"
+    assert "g_sat_fits = false" in body and "!g_sat_fits" in TEXT[TEXT.index("bool serve_attn_tc_supported"):]
