@@ -19,8 +19,9 @@ namespace tlb {
 // One CTA per (query, head): a warp per key in turn, a lane per 16 bytes of the row (C of them where rows are longer than a warp's
 // 512 bytes), f32 products, running maximum and sums per warp, the warps merged through shared memory. Only visible keys are read. A
 // head reads its keys from L2 after the first of its group has. Bound by a warp's chain of load, product, shuffles and exponential per key: one prompt of 333
-// tokens, 32 + 8 heads, takes 189 us at head size 256 and 280 at 512, 1000 tokens of 256 1442 us. Two streams of such rows do not fit the
-// tensor memory beside their scores, so they are not on the tensor-core kernel.
+// tokens, 32 + 8 heads, takes 185 us at head size 256 and 283 at 512, 1000 tokens of 256 1533 us (10 at the tensor cores' rate); 32 sequences x 16 drafts behind 2048
+// tokens 5.9 ms at 256 and 9.3 ms at 512, as keys and values are read again for every draft and query head. Two streams of such rows do not fit the
+// tensor memory beside their scores, so they are not on the tensor-core kernel as it is; one stream with two tiles of 64 scores would fit up to 256.
 template <typename T, bool PAGED, int C>
 __global__ void __launch_bounds__(128) k_serve_attn_any(const ServeAttn a) {
     griddep_launch();

@@ -9,7 +9,7 @@
 //
 // Two streams of S and O per CTA keep the tensor core busy while the exponentials of the other one are taken:
 //   SHARE  a pair of row tiles against every key tile (prompts)
-//   else   one row tile, key tiles in turn; the two O are joined at the end (drafts, chunks of few tokens: bound by the keys' bytes)
+//   else   one row tile, key tiles in turn; the two O are joined at the end (drafts, chunks of few tokens)
 // Each has four warps, a thread per row. The maximum m that a row's exponents refer to moves when a tile's maximum has outgrown it by 2^8
 // (the factor cancels; P stays far inside f16), so O is rescaled rarely. The row sums add P as it was rounded, so a dominant key's rounding
 // cancels.
@@ -22,10 +22,11 @@
 // a warp looks through their values first: rows behind the sequence's end become zero, and so do values that are not finite, which the rows that see
 // them get added afterwards (add_odd_values).
 //
-// What bounds it. Prompts: a 128 x 128 x 16 MMA takes 60 to 75 cycles to issue and execute, which is 62 % of the time of 1 x 8192 tokens (32 + 8 heads of 128: 480 us,
-// 1.15 PFLOP/s while the clock holds, 970 TFLOP/s under the power cap); the rest is the chain of a stream (read S 250 cycles, maximum 400, exponentials 1400, P V and the
-// next Q K 1024) where the other one does not cover it. Drafts: the keys' and values' bytes, pages of 4 KB in random order: 48 sequences x 32 drafts over up to 8192
-// tokens 157 to 169 us = 5.0 to 5.4 TB/s. Short calls: the plan (5000 cycles from the kernel's start to the first copy), an epilogue of 3000 and the joining launch (3 us).
+// What bounds it. Prompts: a 128 x 128 x 16 MMA takes 60 to 75 cycles to issue and execute, which was 62 % of the time of 1 x 8192 tokens (32 + 8 heads of 128) at 480 us
+// (now 488 to 500 us in a graph, 1.10 to 1.13 PFLOP/s while the clock holds, 570 us and 965 TFLOP/s under the power cap); the rest is the chain of a stream (read S 250 cycles,
+// maximum 400, exponentials 1400, P V and the next Q K 1024) where the other one does not cover it. Drafts: 48 sequences x 32 drafts over up to 8192 tokens 167 to 172 us
+// = 4.9 to 5.1 TB/s, 204 us = 4.2 TB/s at 1520 MHz under the power cap. The same with pages of 16, 32, 64 and 128 tokens, and longer as the clock falls: not the pages' bytes but the
+// streams' work per key tile (64 additions more per row and tile within the exponentials: 160 -> 185 us). Short calls: the plan (5000 cycles from the kernel's start to the first copy), an epilogue of 3000 and the joining launch (3 us).
 // Polynomials for some of the exponentials (25, 38, 50 %: 500 us -> 527, 555, 622), P handed over in halves (489 -> 500) and P beside S for heads of 64 (74 -> 82)
 // lost.
 //
@@ -92,7 +93,8 @@ struct Params {
 };
 
 // ---- the line of work
-// sum of floor((a i + b) / m) for 0 <= i < n; a n + b below 2^32
+// sum of floor((a i + b) / m) for 0 <= i < n; a n + b below 2^32. The points under a line, counted as in Euclid's algorithm: whole multiples of m first, what is left with
+// the axes exchanged
 __device__ __forceinline__ int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
     int64_t s = 0;
     while (n > 0) {

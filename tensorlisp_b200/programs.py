@@ -271,7 +271,8 @@ def _layer(g: Graph, cfg: DecoderConfig, wid: dict, i: int, x: int, pos: int, sl
 def packed_prefill_step(cfg: DecoderConfig, n_seqs: int, n_tokens: int, pool_blocks: int) -> DecoderGraph:
     """The prompts of `n_seqs` sequences in one pass, packed one behind the other without padding: `n_tokens` rows hold all of them (rows behind the
     last one are computed and ignored; their cache slots are negative). Inputs: token ids [n_tokens], positions, the offsets [n_seqs + 1] of the
-    prompts, the row index of every prompt's last token, the cache slots. Logits for the last token of every prompt."""
+    prompts, the row index of every prompt's last token, the cache slots. Logits for the last token of every prompt. For one GPU: unlike ``prefill_step``
+    it takes no part of a model that is split over several."""
     g = Graph()
     specs = decoder_weights(cfg)
     wid = {s.name: g.weight(s.ty, s.ne, s.name) for s in specs}
@@ -295,7 +296,7 @@ def verify_step(cfg: DecoderConfig, batch: int, drafts: int, max_ctx: int, pool_
     ids [batch * drafts] (sequence by sequence), their positions (context + depth in the tree), block tables, context lengths, how many
     drafts each sequence has, the drafts' parents [batch, drafts] (-1: the context), the cache slots of the drafts (position context + index of
     the block table; negative for padding), and a token per draft to score. Outputs: the logits of every draft, its argmax, and `scores`
-    (``Graph.token_logprobs`` with `top` alternatives)."""
+    (``Graph.token_logprobs`` with `top` alternatives). For one GPU: unlike ``decoder_step`` it takes no part of a model that is split over several."""
     g = Graph()
     specs = decoder_weights(cfg)
     wid = {s.name: g.weight(s.ty, s.ne, s.name) for s in specs}
